@@ -33,8 +33,12 @@ INDEX_I32, INDEX_I64 = 0, 1
 PACKED_FORMS = ("grouped", "grouped_split", "few_sum", "few_rows", "tiles", "items")
 WEIGHT_F32, WEIGHT_BF16 = 0, 1
 
+DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_F64 = 0, 1, 2, 3
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
+_L = ctypes.c_int64
+_F = ctypes.c_float
 _S = ctypes.c_size_t
 
 # name -> (restype, argtypes)
@@ -99,6 +103,23 @@ _SIGNATURES = {
     "cernels_gpt_oss_moe_experts": (
         ctypes.c_int,
         [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _S, _P],
+    ),
+    "cernels_layer_norm": (ctypes.c_int, [_P, _P, _P, _L, _I, _I, _I, _F, _P, _P, _P]),
+    "cernels_layer_norm_backward_workspace_bytes": (_S, [_L, _I, _I]),
+    "cernels_layer_norm_backward": (ctypes.c_int, [_P, _P, _P, _P, _L, _I, _I, _I, _P, _P, _P, _P, _S, _P]),
+    "cernels_rotary": (
+        ctypes.c_int,
+        [_P, _L, _L, _I, _P, _L, _L, _I, _P, _I, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P],
+    ),
+    "cernels_paged_append": (
+        ctypes.c_int,
+        [_P, _L, _L, _I, _P, _P, _L, _L, _P, _L, _L, _I, _I, _I, _P, _I, _I, _I, _F, _P, _P, _P, _I, _I, _P, _L, _I, _P, _P, _I, _I,
+         _P],
+    ),
+    "cernels_paged_attention_workspace_bytes": (_S, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "cernels_paged_attention": (
+        ctypes.c_int,
+        [_P, _L, _L, _I, _I, _I, _I, _P, _P, _P, _I, _I, _P, _L, _I, _P, _P, _I, _I, _I, _F, _I, _P, _P, _P, _S, _P],
     ),
 }
 

@@ -1,0 +1,621 @@
+// Attention of a step's new tokens over a paged cache. Query head h of token i (position p) of sequence b sees keys j <= p of its
+// sequence, with a window also j > p - window:
+//   o = sum_j e_j v_j / (sum_j e_j + e_sink), e_j = exp(scale q k_j - M), e_sink = exp(sink_h - M)
+// in one pass over the keys with a running M and sum (fp32). A row is one (token, query head of a key head's group); rows of one key
+// head share its keys, so they are the columns of one matrix product S^T = K Q^T.
+//
+// Why S^T: in the matrix instructions' result layout a lane then owns one row of the softmax (a column here), and the values that it
+// holds are exactly the elements that it has to supply as the second operand of O^T = V^T P^T, once the keys of a tile are numbered in
+// the order in which the result registers hold them. The probabilities go from one product to the next without leaving the lane.
+//
+// M is raised only where a new score passes it by kSlack (a factor 2^kSlack in the exponentials, exact in fp32 and harmless in the
+// 16-bit probabilities), so that most tiles need neither a reduction over lanes nor a rescaling of O.
+#include "layer_step.h"
+#include "moe_tile.h"
+
+namespace cmoe {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kSlack = 8.0f;
+constexpr float kNone = -__builtin_inff();
+
+struct MathBf16 {
+    typedef TypeBf16 T;
+    static __device__ __forceinline__ f32x4 mma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) { return pack_bf16x2(a, b); }
+};
+struct MathF16 {
+    typedef TypeF16 T;
+    static __device__ __forceinline__ f32x4 mma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) { return pack_f16x2(a, b); }
+};
+
+// What a launch works on beside the call's own parameters.
+struct AttentionPlan {
+    int splits;    // workgroups that share a tile's keys; above 1 they write partial results
+    int few_rows;  // sequences of at most this many rows take the few-rows kernel, the others the tile kernel; 0: none takes it
+    float* part;   // [tokens * heads][splits][dim] unnormalised O, then [tokens * heads][splits][2] M and sum
+};
+
+__device__ __forceinline__ float2* plan_stats(const AttentionPlan& a, const AttentionParams& p) {
+    return reinterpret_cast<float2*>(a.part + (long long)p.step.tokens * p.q.heads * a.splits * p.dim);
+}
+
+// The part of the keys [begin, end) that split number `i` of `n` takes: whole multiples of `unit`, at least `least` keys a split.
+__device__ __forceinline__ void split_range(int begin, int end, int i, int n, int unit, int least, int& lo, int& hi) {
+    const int keys = end > begin ? end - begin : 0;
+    int per = (keys + n - 1) / n;
+    per = per < least ? least : per;
+    per = (per + unit - 1) / unit * unit;
+    const long long at = (long long)per * i;
+    lo = at < keys ? begin + (int)at : end;
+    hi = end - lo < per ? end : lo + per;
+}
+
+// One row's result: normalised into the output, or as a partial result of its split.
+template <class M>
+__device__ __forceinline__ float row_scale(const AttentionParams& p, int head, float m, float l) {
+    if (p.sinks) l += __builtin_amdgcn_exp2f(p.sinks[head] * kLog2e - (m == kNone ? 0.0f : m));
+    return l > 0.0f || l != l ? 1.0f / l : 0.0f;  // a row that sees nothing is 0
+}
+
+// ---- few rows: single tokens and short chunks ---------------------------------------------------------------------------------
+// Bound by the stream of keys and values. A wave takes 32 keys at a time straight from memory into the operand registers of the
+// 16 x 16 x 32 products, with no LDS between: K's rows as they lie (16 rows x 64 contiguous bytes an instruction), V's rows whole
+// (contiguous), turned by permutes of 16-bit halves within the lane. Four waves of a workgroup share out its keys.
+constexpr int kFewWaves = 4;
+constexpr int kFewKeys = 32;
+
+template <class M, int D, int NT>
+__global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionParams p, AttentionPlan plan) {
+    typedef typename M::T T;
+    typedef typename T::raw raw;
+    constexpr int DS = D / 32;      // steps of the first product
+    constexpr int DJ = D / 16;      // 16-row tiles of the second one's result
+    constexpr int VC = D / 16 / 8 ? D / 128 : 0;  // 16-byte vectors of a V row per lane (0: one 8-byte vector)
+    __shared__ float lds_o[kFewWaves][16 * D];
+    __shared__ float2 lds_ml[kFewWaves][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const int b = blockIdx.z, kh = blockIdx.y;
+    const int group = p.q.heads / p.kv_heads;
+    int first, count;
+    step_tokens(p.step, b, first, count);
+    const int rows = count * group;
+    if (rows == 0 || (plan.few_rows > 0 && rows > plan.few_rows)) return;
+    const int length = p.step.lengths[b];
+    const char* kbase = static_cast<const char*>(p.k.p) + 2 * kh * p.k.head;
+    const char* vbase = static_cast<const char*>(p.v.p) + 2 * kh * p.v.head;
+    const float c = p.scale * kLog2e;
+
+    for (int r0 = 0; r0 < rows; r0 += 16 * NT) {
+        // rows r0 .. r0 + 16 NT - 1: this lane's columns, their queries and the keys that they see
+        u32x4 q[NT][DS];
+        int hi[NT], lo[NT], most_hi = 0, least_lo = 0x7fffffff, all_hi = 0x7fffffff, all_lo = 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int row = r0 + 16 * n + col;
+            const bool live = row < rows;
+            const int token = live ? row / group : 0, head = kh * group + (live ? row - token * group : 0);
+            const raw* src = static_cast<const raw*>(p.q.p) + (first + token) * p.q.token + head * p.q.head;
+#pragma unroll
+            for (int s = 0; s < DS; ++s) q[n][s] = live ? load_vec<T>(src + 8 * (g + 4 * s)) : u32x4{};
+            const int pos = length - count + token;
+            hi[n] = live ? pos + 1 : 0;
+            lo[n] = p.window > 0 && pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
+            if (live) {
+                most_hi = max(most_hi, hi[n]);
+                least_lo = min(least_lo, lo[n]);
+                all_hi = min(all_hi, hi[n]);
+                all_lo = max(all_lo, lo[n]);
+            }
+        }
+#pragma unroll
+        for (int o = 8; o; o >>= 1) {
+            most_hi = max(most_hi, __shfl_xor(most_hi, o));
+            least_lo = min(least_lo, __shfl_xor(least_lo, o));
+            all_hi = min(all_hi, __shfl_xor(all_hi, o));
+            all_lo = max(all_lo, __shfl_xor(all_lo, o));
+        }
+        most_hi = __builtin_amdgcn_readfirstlane(min(most_hi, p.step.blocks * p.step.page_size));
+        least_lo = __builtin_amdgcn_readfirstlane(least_lo);
+        all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+        all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+        int begin, end;
+        split_range(least_lo & ~(kFewKeys - 1), most_hi, blockIdx.x, plan.splits, kFewKeys * kFewWaves, 2 * kFewKeys * kFewWaves, begin, end);
+
+        float m[NT], l[NT];
+        f32x4 o[NT][DJ];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n] = kNone;
+            l[n] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < DJ; ++j) o[n][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        for (int k0 = begin + kFewKeys * wave; k0 < end; k0 += kFewKeys * kFewWaves) {
+            // two runs of 16 keys, each inside one page (pages hold a multiple of 16 keys)
+            u32x4 kr[2][DS];
+            uint32_t vr[8][D / 32];
+            bool bad[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int key = k0 + 16 * u, blk = key / p.step.page_size, slot = key - blk * p.step.page_size;
+                const int page = key < end ? step_page(p.step, b, blk) : -1;
+                bad[u] = page < 0;
+                const long long at = page < 0 ? 0 : page;  // a key that nobody sees is read from page 0 and dropped below
+                const char* kp = kbase + 2 * (at * p.k.page + (slot + col) * p.k.slot);
+#pragma unroll
+                for (int s = 0; s < DS; ++s) kr[u][s] = *reinterpret_cast<const u32x4*>(kp + 16 * (g + 4 * s));
+                const char* vp = vbase + 2 * (at * p.v.page + (slot + 4 * g) * p.v.slot);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const char* row = vp + 2 * i * p.v.slot;
+                    if constexpr (VC == 0) {
+                        const u32x2 t = *reinterpret_cast<const u32x2*>(row + 8 * col);
+                        vr[4 * u + i][0] = t[0], vr[4 * u + i][1] = t[1];
+                    } else {
+#pragma unroll
+                        for (int v = 0; v < VC; ++v) {
+                            const u32x4 t = *reinterpret_cast<const u32x4*>(row + 16 * col + 256 * v);
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) vr[4 * u + i][4 * v + w] = t[w];
+                        }
+                    }
+                }
+            }
+            const bool whole = !bad[0] && !bad[1] && k0 >= all_lo && k0 + kFewKeys <= all_hi && k0 + kFewKeys <= end;
+            if (!whole) {  // values of keys outside the sequence may be anything, and 0 times anything is not always 0
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = k0 + 16 * (i >> 2) + 4 * g + (i & 3);
+                    const bool drop = bad[i >> 2] || key >= end || key < least_lo;
+#pragma unroll
+                    for (int w = 0; w < D / 32; ++w) vr[i][w] = drop ? 0u : vr[i][w];
+                }
+            }
+            u32x4 pr[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                f32x4 s[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int d = 0; d < DS; ++d) s[u] = M::mma16(kr[u][d], q[n][d], s[u]);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int key = k0 + 16 * (i >> 2) + 4 * g + (i & 3);
+                        const bool sees = !bad[i >> 2] && key < hi[n] && key >= lo[n] && key < end;
+                        s[i >> 2][i & 3] = sees ? s[i >> 2][i & 3] : kNone;
+                    }
+                }
+                float t = s[0][0];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) t = fmaxf(t, s[i >> 2][i & 3]);
+                t *= c;
+                if (__ballot(t > m[n] + kSlack) != 0) {
+                    t = fmaxf(t, __shfl_xor(t, 16));
+                    t = fmaxf(t, __shfl_xor(t, 32));
+                    const float m1 = fmaxf(m[n], t);
+                    const float f = m1 == kNone ? 1.0f : __builtin_amdgcn_exp2f(m[n] - m1);
+                    m[n] = m1;
+                    l[n] *= f;
+#pragma unroll
+                    for (int j = 0; j < DJ; ++j) o[n][j] *= f;
+                }
+                const float sub = m[n] == kNone ? 0.0f : m[n];
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], c, -sub));
+                    l[n] += e[i];
+                }
+                // rounded to the values' type for the product, as the sum is not: within half a step of each term
+                pr[n] = u32x4{M::pack2(e[0], e[1]), M::pack2(e[2], e[3]), M::pack2(e[4], e[5]), M::pack2(e[6], e[7])};
+            }
+#pragma unroll
+            for (int j = 0; j < DJ; ++j) {
+                // V^T's rows d = (D / 16) col + j, or 8 col + j % 8 of each 128 where a lane has several vectors
+                const int w = j / 2;
+                const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+                u32x4 a;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(vr[2 * i + 1][w], vr[2 * i][w], sel);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) o[n][j] = M::mma16(a, pr[n], o[n][j]);
+            }
+        }
+        // the waves' results, one set of 16 rows after the other
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            l[n] += __shfl_xor(l[n], 16);
+            l[n] += __shfl_xor(l[n], 32);
+            __syncthreads();
+            if (g == 0) lds_ml[wave][col] = make_float2(m[n], l[n]);
+#pragma unroll
+            for (int j = 0; j < DJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 4 * g + r;  // of V^T's 16: the column that this row's lane loaded
+                    const int d = VC == 0 ? (D / 16) * row + j : 128 * (j / 8) + 8 * row + j % 8;
+                    lds_o[wave][col * D + (d ^ (col & 7) * 4)] = o[n][j][r];
+                }
+            __syncthreads();
+            constexpr int kPer = 64 * kFewWaves / 16;  // threads that share a row
+            const int my = threadIdx.x / kPer, part = threadIdx.x % kPer, row = r0 + 16 * n + my;
+            if (row < rows) {
+                float mx = kNone, sum = 0.0f, f[kFewWaves];
+#pragma unroll
+                for (int w = 0; w < kFewWaves; ++w) mx = fmaxf(mx, lds_ml[w][my].x);
+#pragma unroll
+                for (int w = 0; w < kFewWaves; ++w) {
+                    f[w] = lds_ml[w][my].x == kNone ? 0.0f : __builtin_amdgcn_exp2f(lds_ml[w][my].x - mx);
+                    sum += f[w] * lds_ml[w][my].y;
+                }
+                const int token = row / group, head = kh * group + row - token * group;
+                const long long at = (long long)(first + token) * p.q.heads + head;
+                const float k = plan.splits > 1 ? 1.0f : row_scale<M>(p, head, mx, sum);
+                for (int d = 4 * part; d < D; d += 4 * kPer) {
+                    f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int w = 0; w < kFewWaves; ++w)
+                        v += f[w] * *reinterpret_cast<const f32x4*>(&lds_o[w][my * D + (d ^ (my & 7) * 4)]);
+                    if (plan.splits > 1)
+                        *reinterpret_cast<f32x4*>(plan.part + (at * plan.splits + blockIdx.x) * D + d) = v;
+                    else
+                        *reinterpret_cast<u32x2*>(static_cast<raw*>(p.out) + at * D + d) =
+                            u32x2{M::pack2(v[0] * k, v[1] * k), M::pack2(v[2] * k, v[3] * k)};
+                }
+                if (plan.splits > 1 && part == 0) plan_stats(plan, p)[at * plan.splits + blockIdx.x] = make_float2(mx, sum);
+            }
+        }
+    }
+}
+
+// ---- many rows: chunks and prompts --------------------------------------------------------------------------------------------
+// Bound by the matrix instructions. Four waves of 32 rows each share tiles of keys and values in LDS, the next tile on its way there
+// while one is worked on. K's 16-byte vectors are read as operands as they are; V's operands are columns, which LDS hands out turned
+// (ds_read_b64_tr_b16: 4 keys of one column per lane).
+constexpr int kTileWaves = 4;
+constexpr int kTileRows = 32 * kTileWaves;
+
+template <int D>
+struct TileSize {
+    static constexpr int kKeys = D <= 128 ? 64 : 32;
+    static constexpr int kBytes = kKeys * D * 2;
+};
+
+__device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+// Which tile of which sequence workgroup `i` has: tiles are numbered over the sequences with more than few_rows rows.
+struct TileId {
+    int b, row0, rows, first, count;
+};
+__device__ __forceinline__ bool find_tile(const AttentionParams& p, const AttentionPlan& plan, int i, TileId& t) {
+    const int lane = threadIdx.x & 63, group = p.q.heads / p.kv_heads;
+    for (int b0 = 0; b0 < p.step.seqs; b0 += 64) {
+        const int b = b0 + lane;
+        int first = 0, count = 0;
+        if (b < p.step.seqs) step_tokens(p.step, b, first, count);
+        const int rows = count * group;
+        const int tiles = rows > plan.few_rows ? (rows + kTileRows - 1) / kTileRows : 0;
+        int sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(sum, o);
+            if (lane >= o) sum += up;
+        }
+        const unsigned long long has = __ballot(sum > i);
+        if (has) {
+            const int l = __builtin_ctzll(has);
+            t.b = b0 + l;
+            t.first = __builtin_amdgcn_readlane(first, l);
+            t.count = __builtin_amdgcn_readlane(count, l);
+            t.rows = __builtin_amdgcn_readlane(rows, l);
+            const int before = __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(tiles, l);
+            t.row0 = (i - before) * kTileRows;
+            return true;
+        }
+        i -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
+template <class M, int D>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(AttentionParams p, AttentionPlan plan) {
+    typedef typename M::T T;
+    typedef typename T::raw raw;
+    constexpr int KT = TileSize<D>::kKeys, kBytes = TileSize<D>::kBytes;
+    constexpr int CH = D / 8;               // 16-byte vectors of a row
+    constexpr int kRowsPer = 64 / CH;       // rows that one copy instruction of a wave moves
+    constexpr int kCopies = KT / kRowsPer / kTileWaves;  // per wave, of each of K and V
+    constexpr int DS = D / 16, DT = D / 32, KU = KT / 32;
+    extern __shared__ __align__(1024) unsigned char lds[];  // [2][K | V]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+    const int kh = blockIdx.x % p.kv_heads, group = p.q.heads / p.kv_heads;
+    TileId t;
+    if (!find_tile(p, plan, blockIdx.x / p.kv_heads, t)) return;
+    const int length = p.step.lengths[t.b];
+    const char* kbase = static_cast<const char*>(p.k.p) + 2 * kh * p.k.head;
+    const char* vbase = static_cast<const char*>(p.v.p) + 2 * kh * p.v.head;
+    const float c = p.scale * kLog2e;
+
+    const int row = t.row0 + 32 * wave + col;
+    const bool live = row < t.rows;
+    const int token = live ? row / group : 0, head = kh * group + (live ? row - token * group : 0);
+    u32x4 q[DS];
+    {
+        const raw* src = static_cast<const raw*>(p.q.p) + (t.first + token) * p.q.token + head * p.q.head;
+#pragma unroll
+        for (int s = 0; s < DS; ++s) q[s] = live ? load_vec<T>(src + 16 * s + 8 * h) : u32x4{};
+    }
+    // keys that the row, the wave's rows and the tile's rows see; positions grow with the row
+    const int cap = p.step.blocks * p.step.page_size, before = length - t.count;
+    auto low = [&](int tok) { return p.window > 0 && before + tok - p.window + 1 > 0 ? before + tok - p.window + 1 : 0; };
+    const int hi = live ? before + token + 1 : 0, lo = low(token);
+    const int last_row = min(t.row0 + kTileRows, t.rows) - 1;
+    const int w_first = min(t.row0 + 32 * wave, last_row) / group, w_last = min(t.row0 + 32 * wave + 31, last_row) / group;
+    const bool idle = t.row0 + 32 * wave >= t.rows;
+    const int w_hi = before + w_last + 1, w_all_hi = before + w_first + 1, w_lo = low(w_first), w_all_lo = low(w_last);
+    const int tile_lo = low(t.row0 / group) / KT * KT;
+    const int tile_hi = min(before + last_row / group + 1, cap);
+    int begin, end;
+    split_range(tile_lo, tile_hi, blockIdx.y, plan.splits, KT, 4 * KT, begin, end);
+    const int drop_lo = low(t.row0 / group);
+
+    // One tile's copies: rows past the keys that anybody sees, or without a page, come from zeros (V) or are dropped later (K).
+    const int crow = lane / CH, cpos = lane % CH;
+    auto copy = [&](int k0, int buf) {
+        const uint32_t base = lds_u32(lds) + buf * 2 * kBytes;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int r0 = (wave * kCopies + i) * kRowsPer;  // of the tile, the same in all lanes; its rows lie in one page
+            const int key = k0 + r0, blk = key / p.step.page_size, slot = key - blk * p.step.page_size;
+            const int page = key < end ? step_page(p.step, t.b, blk) : -1;
+            const long long at = page < 0 ? 0 : page;
+            const int r = r0 + crow;
+            const char* kp = kbase + 2 * (at * p.k.page + (slot + crow) * p.k.slot) + 16 * (cpos ^ (r & (CH - 1) & 15));
+            dma16(kp, base + r0 * D * 2);
+            const char* vp = vbase + 2 * (at * p.v.page + (slot + crow) * p.v.slot) + 16 * (cpos ^ (2 * r & (CH - 1) & 15));
+            const bool zero = page < 0 || k0 + r >= end || k0 + r < drop_lo;
+            dma16(zero ? reinterpret_cast<const char*>(kZeros) : vp, base + kBytes + r0 * D * 2);
+        }
+    };
+
+    float m = kNone, l = 0.0f;
+    f32x16 o[DT];
+#pragma unroll
+    for (int j = 0; j < DT; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[j][i] = 0.0f;
+
+    int buf = 0;
+    if (begin < end) copy(begin, 0);
+    for (int k0 = begin; k0 < end; k0 += KT, buf ^= 1) {
+        wait_vmcnt<0>();
+        __syncthreads();
+        if (k0 + KT < end) copy(k0 + KT, buf ^ 1);
+        if (idle || k0 >= w_hi || k0 + KT <= w_lo) continue;
+        const unsigned char* kt = lds + buf * 2 * kBytes;
+        const uint32_t vt = lds_u32(kt) + kBytes;
+        f32x16 s[KU];
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+            const int r = 32 * u + col;
+#pragma unroll
+            for (int d = 0; d < DS; ++d) {
+                const u32x4 a = *reinterpret_cast<const u32x4*>(kt + r * D * 2 + 16 * ((2 * d + h) ^ (r & (CH - 1) & 15)));
+                s[u] = M::mma32(a, q[d], s[u]);
+            }
+        }
+        bool whole = k0 >= w_all_lo && k0 + KT <= w_all_hi && k0 + KT <= end;
+        uint32_t pages_bad = 0;  // bit r / 16: the 16 keys have no page
+#pragma unroll
+        for (int r = 0; r < KT; r += 16) {
+            const int blk = (k0 + r) / p.step.page_size;
+            if (k0 + r < end && step_page(p.step, t.b, blk) < 0) pages_bad |= 1u << (r / 16);
+        }
+        if (pages_bad) whole = false;
+        if (!whole) {
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3), key = k0 + r;
+                    const bool sees = key < hi && key >= lo && key < end && !(pages_bad >> (r / 16) & 1);
+                    s[u][i] = sees ? s[u][i] : kNone;
+                }
+        }
+        float x = s[0][0];
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x = fmaxf(x, s[u][i]);
+        x *= c;
+        if (__ballot(x > m + kSlack) != 0) {
+            const float m1 = fmaxf(m, max_halves(x));
+            const float f = m1 == kNone ? 1.0f : __builtin_amdgcn_exp2f(m - m1);
+            m = m1;
+            l *= f;
+#pragma unroll
+            for (int j = 0; j < DT; ++j) o[j] *= f;
+        }
+        const float sub = m == kNone ? 0.0f : m;
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * k + i], c, -sub));
+                    l += e[i];
+                }
+                const u32x4 pr{M::pack2(e[0], e[1]), M::pack2(e[2], e[3]), M::pack2(e[4], e[5]), M::pack2(e[6], e[7])};
+#pragma unroll
+                for (int j = 0; j < DT; ++j) {
+                    u32x4 a;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        // 4 keys x 16 columns for each 16 lanes: lane n of them addresses 4 columns of key n / 4 and gets column n
+                        const int r = 32 * u + 16 * k + 8 * i + 4 * h + (lane & 15) / 4;
+                        const int chunk = 4 * j + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                        const uint32_t at = vt + r * D * 2 + 16 * (chunk ^ (2 * r & (CH - 1) & 15)) + 8 * (lane & 1);
+                        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+                        const u32x2 w = __builtin_bit_cast(u32x2, v);
+                        a[2 * i] = w[0], a[2 * i + 1] = w[1];
+                    }
+                    o[j] = M::mma32(a, pr, o[j]);
+                }
+            }
+    }
+    {
+        uint32_t a = __float_as_uint(l), b = a;
+        swap_halves(a, b);
+        l = __uint_as_float(a) + __uint_as_float(b);
+    }
+    if (!live) return;
+    const long long at = (long long)(t.first + token) * p.q.heads + head;
+    if (plan.splits > 1) {
+        if (h == 0) plan_stats(plan, p)[at * plan.splits + blockIdx.y] = make_float2(m, l);
+        float* part = plan.part + (at * plan.splits + blockIdx.y) * D;
+        if (l == 0.0f) return;  // nobody reads it
+#pragma unroll
+        for (int j = 0; j < DT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4*>(part + 32 * j + 8 * i + 4 * h) =
+                    f32x4{o[j][4 * i], o[j][4 * i + 1], o[j][4 * i + 2], o[j][4 * i + 3]};
+        return;
+    }
+    const float k = row_scale<M>(p, head, m, l);
+    raw* out = static_cast<raw*>(p.out) + at * D;
+#pragma unroll
+    for (int j = 0; j < DT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<u32x2*>(out + 32 * j + 8 * i + 4 * h) = u32x2{M::pack2(o[j][4 * i] * k, o[j][4 * i + 1] * k),
+                                                                            M::pack2(o[j][4 * i + 2] * k, o[j][4 * i + 3] * k)};
+}
+
+// ---- joining the splits ---------------------------------------------------------------------------------------------------------
+// One wave per row: the splits' M and sums by lane, then the O of those that saw a key, in their order.
+template <class M, int D>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttentionParams p, AttentionPlan plan) {
+    typedef typename M::T::raw raw;
+    constexpr int E = D / 64;
+    const int lane = threadIdx.x & 63;
+    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int token = (int)(at / p.q.heads), head = (int)(at - (long long)token * p.q.heads);
+    if (token >= p.step.tokens) return;
+    if (step_sequence(p.step, token) >= p.step.seqs) return;
+    const float2* st = plan_stats(plan, p) + at * plan.splits;
+    const float2 mine = lane < plan.splits ? st[lane] : make_float2(kNone, 0.0f);
+    const float mx = wave_max(mine.y == 0.0f ? kNone : mine.x);
+    const float f = mine.y == 0.0f || mine.x == kNone ? 0.0f : __builtin_amdgcn_exp2f(mine.x - mx);
+    const float sum = wave_sum(f * mine.y);
+    const unsigned long long used = __ballot(mine.y != 0.0f);
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+    const float* part = plan.part + at * plan.splits * D;
+    for (unsigned long long left = used; left; left &= left - 1) {
+        const int i = __builtin_ctzll(left);
+        const float w = __shfl(f, i);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += w * part[(long long)i * D + E * lane + e];
+    }
+    const float k = row_scale<M>(p, head, mx, sum);
+    raw* out = static_cast<raw*>(p.out) + at * D + E * lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e] = M::T::put(o[e] * k);
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------------
+
+bool attention_dim_ok(int dim) { return dim == 64 || dim == 128 || dim == 256; }
+
+constexpr int kMostSplits = 64;  // the join kernel holds a split's statistics per lane
+constexpr int kFewMost = 32;     // rows of a sequence that the few-rows kernel takes in one pass over its keys
+
+struct Forms {
+    bool few, tile;
+    int splits, tiles;
+    long long most;  // rows of the sequence with the most of them, as far as the caller says
+};
+
+static Forms attention_forms(const AttentionParams& p) {
+    const int group = p.q.heads / p.kv_heads;
+    const long long rows = (long long)p.step.tokens * group;
+    const long long keys = (long long)p.step.blocks * p.step.page_size;
+    const int even = (p.step.tokens + p.step.seqs - 1) / p.step.seqs;  // some sequence has at least that many tokens
+    Forms f{};
+    f.most = (long long)(p.max_new > p.step.tokens ? p.step.tokens : p.max_new < even ? even : p.max_new) * group;
+    f.tile = f.most > kFewMost;
+    f.few = !f.tile || p.step.seqs > 1;
+    // many-row sequences: at most one partly filled tile each
+    const long long seqs = p.step.seqs < rows / (kFewMost + 1) ? p.step.seqs : rows / (kFewMost + 1);
+    f.tiles = f.tile ? (int)((rows + kTileRows - 1) / kTileRows + seqs) : 0;
+    const long long groups = f.tile ? (long long)f.tiles * p.kv_heads : (long long)p.step.seqs * p.kv_heads;
+    const long long want = (f.tile ? 512 : f.most > 16 ? 2048 : 4096) / groups;
+    const long long useful = (keys + 255) / 256;
+    const long long n = want < useful ? want : useful;
+    f.splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+    return f;
+}
+
+size_t attention_workspace_bytes(const AttentionParams& p) {
+    const Forms f = attention_forms(p);
+    if (f.splits <= 1) return 16;
+    return (size_t)p.step.tokens * p.q.heads * f.splits * (p.dim + 2) * sizeof(float);
+}
+
+template <class M, int D>
+static hipError_t attention_d(const AttentionParams& p, hipStream_t s) {
+    const Forms f = attention_forms(p);
+    AttentionPlan plan{f.splits, f.tile ? kFewMost : 0, p.ws};
+    if (f.tile) {
+        const int lds = 4 * TileSize<D>::kBytes;
+        if (!f.few) plan.few_rows = 0;
+        hipLaunchKernelGGL((attend_tile_kernel<M, D>), dim3(f.tiles * p.kv_heads, f.splits), dim3(64 * kTileWaves), lds, s, p, plan);
+    }
+    if (f.few) {
+        const dim3 grid(f.splits, p.kv_heads, p.step.seqs);
+        if (f.most <= 16) hipLaunchKernelGGL((attend_few_kernel<M, D, 1>), grid, dim3(64 * kFewWaves), 0, s, p, plan);
+        else hipLaunchKernelGGL((attend_few_kernel<M, D, 2>), grid, dim3(64 * kFewWaves), 0, s, p, plan);
+    }
+    if (f.splits > 1) {
+        const long long rows = (long long)p.step.tokens * p.q.heads;
+        hipLaunchKernelGGL((attend_join_kernel<M, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p, plan);
+    }
+    return hipGetLastError();
+}
+
+template <class M>
+static hipError_t attention_m(const AttentionParams& p, hipStream_t s) {
+    if (p.dim == 64) return attention_d<M, 64>(p, s);
+    if (p.dim == 128) return attention_d<M, 128>(p, s);
+    return attention_d<M, 256>(p, s);
+}
+
+hipError_t launch_attention(const AttentionParams& p, hipStream_t s) {
+    return p.dtype == kDtBf16 ? attention_m<MathBf16>(p, s) : attention_m<MathF16>(p, s);
+}
+
+}  // namespace cmoe

@@ -1,0 +1,452 @@
+// Layer norm, forward and backward.
+//   m = mean x, r = 1 / sqrt(mean (x - m)^2 + eps), h = (x - m) r, y = h w + b
+//   g = dy w, dx = r (g - mean g - h mean(g h)), dw = sum over rows of dy h, db = sum over rows of dy
+// All sums are fp32. Both passes are bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.
+//
+// One to eight waves hold a row in registers, a few 16-byte vectors per lane, so that a row is read once and its variance is taken
+// about its mean; one wave per row needs no barrier. Wider rows take one workgroup each and read the row again from L2.
+// Backward keeps the columns' sums of dw and db in registers over the rows that a lane sees, adds the rows of a workgroup through LDS
+// in order and writes one partial row per workgroup; a second launch adds those in order: no atomics, the same bits every run.
+#include "layer_common.h"
+
+namespace cmoe {
+
+constexpr int kWaves = 8;       // of a workgroup, shared out over its rows
+constexpr int kRowChunks = 4;   // vectors of a row per lane, forward
+constexpr int kBackChunks = 3;  // backward: two rows' vectors and two sums per column; 128 registers leave 16 waves to a CU
+constexpr int kWideThreads = 1024;
+
+// Vector c of a row, zeros past its end.
+template <class T>
+__device__ __forceinline__ u32x4 row_load(const typename T::raw* __restrict__ row, int c, int cols) {
+    const int at = c * T::kVec;
+    if (at + T::kVec <= cols) return load_vec<T>(row + at);
+    float f[T::kVec];
+#pragma unroll
+    for (int i = 0; i < T::kVec; ++i) f[i] = at + i < cols ? T::get(row[at + i]) : 0.0f;
+    return T::pack(f);
+}
+
+template <class T>
+__device__ __forceinline__ void row_store(typename T::raw* __restrict__ row, int c, int cols, const float* f) {
+    const int at = c * T::kVec;
+    if (at + T::kVec <= cols) {
+        store_vec<T>(row + at, T::pack(f));
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < T::kVec; ++i)
+        if (at + i < cols) row[at + i] = T::put(f[i]);
+}
+
+// N values of a column vector (weight or bias, in the rows' type or fp32) from column `at`; 0 past its end.
+template <class W, int N>
+__device__ __forceinline__ void cols_load(const typename W::raw* __restrict__ w, int at, int cols, float* f) {
+    if (at + N <= cols) {
+#pragma unroll
+        for (int i = 0; i < N; i += W::kVec) W::unpack(load_vec<W>(w + at + i), f + i);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = at + i < cols ? W::get(w[at + i]) : 0.0f;
+}
+
+// Sums over the `gw` waves that share a row, of N values a thread; every thread of the row returns the totals. `lds` holds N floats
+// per wave and is not written again before the next barrier. Waves of one row add in their order.
+template <int N>
+__device__ __forceinline__ void row_sum(float* v, int gw, float* lds) {
+    const int wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = wave_sum(v[n]);
+    if (gw == 1) return;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) lds[wave * N + n] = v[n];
+    }
+    __syncthreads();
+    const int first = wave & ~(gw - 1);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        v[n] = 0.0f;
+        for (int w = 0; w < gw; ++w) v[n] += lds[(first + w) * N + n];
+    }
+}
+
+template <class T, class W, int NC>
+__global__ __launch_bounds__(64 * kWaves) void norm_row_kernel(NormParams p, int gw) {
+    constexpr int V = T::kVec;
+    __shared__ float lds[2][kWaves];
+    const int wave = threadIdx.x >> 6, groups = kWaves / gw;
+    const long long row = (long long)blockIdx.x * groups + wave / gw;
+    const int cols = row < p.rows ? p.cols : 0;  // a row past the last one reads and writes nothing
+    const int first = (wave & (gw - 1)) * 64 + (threadIdx.x & 63), step = 64 * gw;
+    const typename T::raw* x = static_cast<const typename T::raw*>(p.x) + row * cols;
+    u32x4 raw[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) raw[c] = row_load<T>(x, c * step + first, cols);
+    float sum[1] = {0.0f};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        float f[V];
+        T::unpack(raw[c], f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[0] += f[i];
+    }
+    const float inv = 1.0f / (float)p.cols;
+    row_sum<1>(sum, gw, lds[0]);
+    const float mean = sum[0] * inv;
+    sum[0] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        float f[V];
+        T::unpack(raw[c], f);
+        const int at = (c * step + first) * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float d = at + i < cols ? f[i] - mean : 0.0f;
+            sum[0] += d * d;
+        }
+    }
+    row_sum<1>(sum, gw, lds[1]);
+    const float rstd = 1.0f / sqrtf(sum[0] * inv + p.eps);
+    if (p.stats && first == 0 && cols) p.stats[2 * row] = mean, p.stats[2 * row + 1] = rstd;
+    typename T::raw* y = static_cast<typename T::raw*>(p.y) + row * cols;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int at = (c * step + first) * V;
+        if (at < cols) {
+            float f[V], w[V], b[V];
+            T::unpack(raw[c], f);
+            cols_load<W, V>(static_cast<const typename W::raw*>(p.weight), at, cols, w);
+            if (p.bias) {
+                cols_load<W, V>(static_cast<const typename W::raw*>(p.bias), at, cols, b);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) b[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = (f[i] - mean) * rstd * w[i] + b[i];
+            row_store<T>(y, c * step + first, cols, f);
+        }
+    }
+}
+
+// Sum over a workgroup of N values a thread; every thread returns the totals. `lds` holds N floats per wave.
+template <int N>
+__device__ __forceinline__ void block_sum(float* v, float* lds) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        v[n] = wave_sum(v[n]);
+        if (lane == 0) lds[wave * N + n] = v[n];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        float t = 0.0f;
+        for (int w = 0; w < waves; ++w) t += lds[w * N + n];
+        v[n] = t;
+    }
+    __syncthreads();
+}
+
+template <class T, class W>
+__global__ __launch_bounds__(kWideThreads) void norm_wide_kernel(NormParams p) {
+    constexpr int V = T::kVec;
+    __shared__ float lds[kWideThreads / 64];
+    const int cols = p.cols, chunks = ceil_div(cols, V);
+    const float inv = 1.0f / (float)cols;
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const typename T::raw* x = static_cast<const typename T::raw*>(p.x) + row * cols;
+        float s[1] = {0.0f};
+        for (int c = threadIdx.x; c < chunks; c += kWideThreads) {
+            float f[V];
+            T::unpack(row_load<T>(x, c, cols), f);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[0] += f[i];
+        }
+        block_sum<1>(s, lds);
+        const float mean = s[0] * inv;
+        s[0] = 0.0f;
+        for (int c = threadIdx.x; c < chunks; c += kWideThreads) {
+            float f[V];
+            T::unpack(row_load<T>(x, c, cols), f);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = c * V + i < cols ? f[i] - mean : 0.0f;
+                s[0] += d * d;
+            }
+        }
+        block_sum<1>(s, lds);
+        const float rstd = 1.0f / sqrtf(s[0] * inv + p.eps);
+        if (p.stats && threadIdx.x == 0) p.stats[2 * row] = mean, p.stats[2 * row + 1] = rstd;
+        typename T::raw* y = static_cast<typename T::raw*>(p.y) + row * cols;
+        for (int c = threadIdx.x; c < chunks; c += kWideThreads) {
+            float f[V], w[V], b[V];
+            T::unpack(row_load<T>(x, c, cols), f);
+            cols_load<W, V>(static_cast<const typename W::raw*>(p.weight), c * V, cols, w);
+            if (p.bias) {
+                cols_load<W, V>(static_cast<const typename W::raw*>(p.bias), c * V, cols, b);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) b[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = (f[i] - mean) * rstd * w[i] + b[i];
+            row_store<T>(y, c, cols, f);
+        }
+    }
+}
+
+// Workgroups of the backward pass: two per CU where the rows are many (every workgroup's sums are a partial row that is written and
+// read once more), else one per `groups` rows.
+constexpr int kBackBlocks = 512;
+
+template <class T, class W, int NC>
+__global__ __launch_bounds__(64 * kWaves) void norm_back_kernel(NormParams p, int gw) {
+    constexpr int V = T::kVec;
+    extern __shared__ float sums[];  // [NC * gw * 64 * V], at most 48 KB
+    __shared__ float lds[2][2 * kWaves];
+    const int wave = threadIdx.x >> 6, groups = kWaves / gw, group = wave / gw;
+    const int first = (wave & (gw - 1)) * 64 + (threadIdx.x & 63), step = 64 * gw;
+    const int cols = p.cols;
+    const float inv = 1.0f / (float)cols;
+    float dw[NC][V], db[NC][V];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < V; ++i) dw[c][i] = db[c][i] = 0.0f;
+    int turn = 0;
+    for (long long r0 = (long long)blockIdx.x * groups; r0 < p.rows; r0 += (long long)gridDim.x * groups, turn ^= 1) {
+        const long long row = r0 + group;
+        const bool live = row < p.rows;  // the other rows of the workgroup still meet at its barrier
+        const int n = live ? cols : 0;
+        const typename T::raw* x = static_cast<const typename T::raw*>(p.x) + row * n;
+        const typename T::raw* dy = static_cast<const typename T::raw*>(p.dy) + row * n;
+        u32x4 xr[NC], gr[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            xr[c] = row_load<T>(x, c * step + first, n);
+            gr[c] = row_load<T>(dy, c * step + first, n);
+        }
+        const float mean = live ? p.stats[2 * row] : 0.0f, rstd = live ? p.stats[2 * row + 1] : 0.0f;
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int at = (c * step + first) * V;
+            if (at < n) {
+                float f[V], g[V], w[V];
+                T::unpack(xr[c], f);
+                T::unpack(gr[c], g);
+                cols_load<W, V>(static_cast<const typename W::raw*>(p.weight), at, n, w);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float h = (f[i] - mean) * rstd;
+                    const float gw_ = g[i] * w[i];  // 0 past the row's end, where dy and w are read as 0
+                    dw[c][i] += g[i] * h;
+                    db[c][i] += g[i];
+                    s[0] += gw_;
+                    s[1] += gw_ * h;
+                }
+            }
+        }
+        if (!p.dx) continue;
+        row_sum<2>(s, gw, lds[turn]);  // turns alternate: a wave may still read one row's sums while another writes the next row's
+        s[0] *= inv;
+        s[1] *= inv;
+        typename T::raw* dx = static_cast<typename T::raw*>(p.dx) + row * n;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int at = (c * step + first) * V;
+            if (at < n) {
+                float f[V], g[V], w[V];
+                T::unpack(xr[c], f);
+                T::unpack(gr[c], g);
+                cols_load<W, V>(static_cast<const typename W::raw*>(p.weight), at, n, w);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float h = (f[i] - mean) * rstd;
+                    f[i] = rstd * (g[i] * w[i] - s[0] - h * s[1]);
+                }
+                row_store<T>(dx, c * step + first, n, f);
+            }
+        }
+    }
+    if (!p.partial) return;
+    const int width = NC * step;
+    float* part = p.partial + (long long)blockIdx.x * 2 * cols;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        for (int t = 0; t < groups; ++t) {
+            __syncthreads();
+            if (group == t) {
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const int at = i * width + c * step + first;  // consecutive lanes on consecutive banks
+                        const float v = which ? db[c][i] : dw[c][i];
+                        sums[at] = t ? sums[at] + v : v;
+                    }
+            }
+        }
+        __syncthreads();
+        for (int j = threadIdx.x; j < cols; j += 64 * kWaves) part[which * cols + j] = sums[(j % V) * width + j / V];
+    }
+}
+
+// Rows too wide for a wave's registers: dx by one workgroup per row, the columns' sums by strips of columns.
+template <class T, class W>
+__global__ __launch_bounds__(kWideThreads) void norm_back_wide_kernel(NormParams p) {
+    constexpr int V = T::kVec;
+    __shared__ float lds[2 * kWideThreads / 64];
+    const int cols = p.cols, chunks = ceil_div(cols, V);
+    const float inv = 1.0f / (float)cols;
+    const typename W::raw* weight = static_cast<const typename W::raw*>(p.weight);
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const typename T::raw* x = static_cast<const typename T::raw*>(p.x) + row * cols;
+        const typename T::raw* dy = static_cast<const typename T::raw*>(p.dy) + row * cols;
+        const float mean = p.stats[2 * row], rstd = p.stats[2 * row + 1];
+        float s[2] = {0.0f, 0.0f};
+        for (int c = threadIdx.x; c < chunks; c += kWideThreads) {
+            float f[V], g[V], w[V];
+            T::unpack(row_load<T>(x, c, cols), f);
+            T::unpack(row_load<T>(dy, c, cols), g);
+            cols_load<W, V>(weight, c * V, cols, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                s[0] += g[i] * w[i];
+                s[1] += g[i] * w[i] * (f[i] - mean) * rstd;
+            }
+        }
+        block_sum<2>(s, lds);
+        typename T::raw* dx = static_cast<typename T::raw*>(p.dx) + row * cols;
+        for (int c = threadIdx.x; c < chunks; c += kWideThreads) {
+            float f[V], g[V], w[V];
+            T::unpack(row_load<T>(x, c, cols), f);
+            T::unpack(row_load<T>(dy, c, cols), g);
+            cols_load<W, V>(weight, c * V, cols, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = rstd * (g[i] * w[i] - s[0] * inv - (f[i] - mean) * rstd * s[1] * inv);
+            row_store<T>(dx, c, cols, f);
+        }
+    }
+}
+
+// Partial row blockIdx.y holds the sums over rows blockIdx.y, blockIdx.y + gridDim.y, ...
+template <class T>
+__global__ __launch_bounds__(256) void norm_strip_kernel(NormParams p) {
+    const int j = blockIdx.x * 256 + threadIdx.x;
+    if (j >= p.cols) return;
+    float dw = 0.0f, db = 0.0f;
+    for (long long row = blockIdx.y; row < p.rows; row += gridDim.y) {
+        const float g = T::get(static_cast<const typename T::raw*>(p.dy)[row * p.cols + j]);
+        const float h = (T::get(static_cast<const typename T::raw*>(p.x)[row * p.cols + j]) - p.stats[2 * row]) * p.stats[2 * row + 1];
+        dw += g * h;
+        db += g;
+    }
+    float* part = p.partial + (long long)blockIdx.y * 2 * p.cols;
+    part[j] = dw;
+    part[p.cols + j] = db;
+}
+
+// dweight and dbias from the partial rows, in their order: 16 threads a column take every 16th row each, then one adds the 16.
+template <class W>
+__global__ __launch_bounds__(1024) void norm_fold_kernel(NormParams p, int rows) {
+    __shared__ float lds[16][65];
+    const int col = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+    const int which = blockIdx.y;  // 0: dweight, 1: dbias
+    float v = 0.0f;
+    if (col < p.cols)
+        for (int r = part; r < rows; r += 16) v += p.partial[((long long)r * 2 + which) * p.cols + col];
+    lds[part][threadIdx.x & 63] = v;
+    __syncthreads();
+    void* out = which ? p.dbias : p.dweight;
+    if (part || col >= p.cols || !out) return;
+    v = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v += lds[r][threadIdx.x & 63];
+    static_cast<typename W::raw*>(out)[col] = W::put(v);
+}
+
+static int vec_of(int dtype) { return dtype == kDtF32 ? 4 : 8; }
+
+// Waves that share a row, so that each lane holds at most `most` vectors of it; 0 where a workgroup's waves do not suffice.
+static int row_waves(int cols, int vec, int most) {
+    for (int gw = 1; gw <= kWaves; gw *= 2)
+        if (ceil_div(ceil_div(cols, vec), 64 * gw) <= most) return gw;
+    return 0;
+}
+static int back_blocks(long long rows, int gw) {
+    const int groups = kWaves / gw;
+    const long long need = (rows + groups - 1) / groups;
+    return (int)(need < 1 ? 1 : need < kBackBlocks ? need : kBackBlocks);
+}
+
+int norm_backward_partials(long long rows, int cols, int dtype) {
+    const int gw = row_waves(cols, vec_of(dtype), kBackChunks);
+    return gw ? back_blocks(rows, gw) : (int)(rows < 1 ? 1 : rows < 64 ? rows : 64);
+}
+
+template <class T, class W>
+static void norm_forward(const NormParams& p, hipStream_t s) {
+    const int gw = row_waves(p.cols, T::kVec, kRowChunks);
+    if (!gw) {
+        const unsigned grid = (unsigned)(p.rows < 4096 ? p.rows : 4096);
+        hipLaunchKernelGGL((norm_wide_kernel<T, W>), dim3(grid), dim3(kWideThreads), 0, s, p);
+        return;
+    }
+    const int nc = ceil_div(ceil_div(p.cols, T::kVec), 64 * gw), groups = kWaves / gw;
+    const dim3 grid((unsigned)((p.rows + groups - 1) / groups));
+#define CMOE_NORM(NC) hipLaunchKernelGGL((norm_row_kernel<T, W, NC>), grid, dim3(64 * kWaves), 0, s, p, gw)
+    if (nc <= 1) CMOE_NORM(1);
+    else if (nc == 2) CMOE_NORM(2);
+    else if (nc == 3) CMOE_NORM(3);
+    else CMOE_NORM(4);
+#undef CMOE_NORM
+}
+
+template <class T, class W>
+static void norm_backward(const NormParams& p, hipStream_t s) {
+    const int gw = row_waves(p.cols, T::kVec, kBackChunks);
+    const int parts = norm_backward_partials(p.rows, p.cols, p.dtype);
+    const bool sums = p.dweight || p.dbias;
+    if (p.rows > 0 && !gw) {
+        const unsigned grid = (unsigned)(p.rows < 4096 ? p.rows : 4096);
+        if (p.dx) hipLaunchKernelGGL((norm_back_wide_kernel<T, W>), dim3(grid), dim3(kWideThreads), 0, s, p);
+        if (sums) hipLaunchKernelGGL((norm_strip_kernel<T>), dim3(ceil_div(p.cols, 256), parts), dim3(256), 0, s, p);
+    } else if (gw) {  // without rows the partial sums are written as zeros
+        NormParams q = p;
+        if (!sums) q.partial = nullptr;
+        const int nc = ceil_div(ceil_div(p.cols, T::kVec), 64 * gw);
+#define CMOE_BACK(NC)                                                                                                  \
+    hipLaunchKernelGGL((norm_back_kernel<T, W, NC>), dim3(parts), dim3(64 * kWaves), sums ? 4 * NC * gw * 64 * T::kVec : 0, s, q, gw)
+        if (nc <= 1) CMOE_BACK(1);
+        else if (nc == 2) CMOE_BACK(2);
+        else CMOE_BACK(3);
+#undef CMOE_BACK
+    } else if (sums) {
+        hipLaunchKernelGGL((norm_strip_kernel<T>), dim3(ceil_div(p.cols, 256), parts), dim3(256), 0, s, p);
+    }
+    if (sums) hipLaunchKernelGGL((norm_fold_kernel<W>), dim3(ceil_div(p.cols, 64), p.dbias ? 2 : 1), dim3(1024), 0, s, p, parts);
+}
+
+hipError_t launch_norm(const NormParams& p, hipStream_t s) {
+    if (p.dtype == kDtF32) norm_forward<TypeF32, TypeF32>(p, s);
+    else if (p.dtype == kDtF16 && p.wdtype == kDtF16) norm_forward<TypeF16, TypeF16>(p, s);
+    else if (p.dtype == kDtF16) norm_forward<TypeF16, TypeF32>(p, s);
+    else if (p.wdtype == kDtBf16) norm_forward<TypeBf16, TypeBf16>(p, s);
+    else norm_forward<TypeBf16, TypeF32>(p, s);
+    return hipGetLastError();
+}
+
+hipError_t launch_norm_backward(const NormParams& p, hipStream_t s) {
+    if (p.dtype == kDtF32) norm_backward<TypeF32, TypeF32>(p, s);
+    else if (p.dtype == kDtF16 && p.wdtype == kDtF16) norm_backward<TypeF16, TypeF16>(p, s);
+    else if (p.dtype == kDtF16) norm_backward<TypeF16, TypeF32>(p, s);
+    else if (p.wdtype == kDtBf16) norm_backward<TypeBf16, TypeBf16>(p, s);
+    else norm_backward<TypeBf16, TypeF32>(p, s);
+    return hipGetLastError();
+}
+
+}  // namespace cmoe

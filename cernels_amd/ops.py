@@ -17,8 +17,10 @@ import ctypes
 import torch
 
 from cernels_amd import _native
+from cernels_amd._call import launch as _launch, require as _require, stream as _stream
 from cernels_amd._native import (ACT_GELU_TANH, ACT_GPTOSS, ACT_RELU, ACT_SILU, ACT_SILU_PLAIN, LAYOUT_CONCAT,
                                  LAYOUT_INTERLEAVED, ROUTER_SOFTMAX_TOPK, ROUTER_TOPK_SOFTMAX, check)
+from cernels_amd.layer_ops import layer_norm, paged_append, paged_attention, rotary, rotary_frequencies
 
 # megablocks_moe's act_id (src/kops/registry/megablocks_moe.py:7 names them; csrc/megablocks_moe.cu:78-96)
 # -> the library's non-gated activation
@@ -29,25 +31,10 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 # The native entries read a router's own types; anything else is converted before the call.
 _INDEX_TYPES = {torch.int32: _native.INDEX_I32, torch.int64: _native.INDEX_I64}
 _WEIGHT_TYPES = {torch.float32: _native.WEIGHT_F32, torch.bfloat16: _native.WEIGHT_BF16}
 _BF16 = torch.bfloat16
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: _stream(torch.device("cuda", i)))
-
-
-def _launch(what: str, device_index: int, fn, *args) -> None:
-    """One native call on the current stream of the tensors' device, which is made current where it is not."""
-    if torch.cuda.current_device() == device_index:
-        st = fn(*args, _raw_stream(device_index))
-    else:
-        with torch.cuda.device(device_index):
-            st = fn(*args, _raw_stream(device_index))
-    check(st, what)
 
 
 def routing(top_k_index: torch.Tensor, top_k_weights: torch.Tensor):
@@ -59,11 +46,6 @@ def routing(top_k_index: torch.Tensor, top_k_weights: torch.Tensor):
             idx = (idx if idx.dtype in _INDEX_TYPES else idx.to(torch.int32)).contiguous()
             w = (w if w.dtype in _WEIGHT_TYPES else w.float()).contiguous()
     return idx, w
-
-
-def _require(cond: bool, msg: str) -> None:
-    if not cond:
-        raise RuntimeError(msg)
 
 
 def _usable(t, dtype, device_index: int, shape) -> bool:
@@ -618,6 +600,7 @@ def megablocks_moe(x, w1, w2, indices, weights, topk, act_id):
 
 
 __all__ = [
+    "layer_norm", "rotary", "rotary_frequencies", "paged_append", "paged_attention",
     "moe_experts", "route", "decode_supported", "PackedExperts", "pack_weights", "pack_experts", "moe_experts_packed",
     "experts_packed", "experts_decode", "moe_block", "routing",
     "cohere2_moe_experts", "cohere2_moe_experts_decode",

@@ -281,6 +281,66 @@ int cernels_gpt_oss_moe_experts(const void* x, const void* gate_up_proj, const f
                                 int32_t topk, void* out, void* workspace, size_t workspace_bytes,
                                 hipStream_t stream);
 
+/* ---- the decoder layer around the experts --------------------------------------------------------
+ * Layer norm, rotary positions, the write of new keys and values into a paged cache and attention over it.
+ * dtype names the element type of a call's tensors; fp64 is for inverse frequencies only. */
+enum cernels_dtype { CERNELS_DTYPE_BF16 = 0, CERNELS_DTYPE_F16 = 1, CERNELS_DTYPE_F32 = 2, CERNELS_DTYPE_F64 = 3 };
+
+/* y = (x - mean) / sqrt(var + eps) * weight (+ bias) over rows of x [rows, cols], contiguous; sums in fp32. weight and bias
+ * (nullable) have the rows' type or fp32 (weight_dtype). stats [rows, 2] (nullable) gets each row's mean and 1 / sqrt(var + eps),
+ * which the backward entry reads. Limits: rows < 2^31, cols <= 2^24; element alignment only. */
+int cernels_layer_norm(const void* x, const void* weight, const void* bias, int64_t rows, int32_t cols, int32_t dtype,
+                       int32_t weight_dtype, float eps, void* y, float* stats, hipStream_t stream);
+/* Gradients for dy [rows, cols]: dx [rows, cols], dweight [cols], dbias [cols] (weight_dtype), each nullable. Deterministic. */
+size_t cernels_layer_norm_backward_workspace_bytes(int64_t rows, int32_t cols, int32_t dtype);
+int cernels_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* stats, int64_t rows, int32_t cols,
+                                int32_t dtype, int32_t weight_dtype, void* dx, void* dweight, void* dbias, void* workspace,
+                                size_t workspace_bytes, hipStream_t stream);
+
+/* Rotary positions on q [tokens, q_heads, dim] and k [tokens, k_heads, dim] (each nullable; last dimension contiguous, token and
+ * head strides in elements): pair i of a head's first 2 * pairs elements, elements 2i and 2i + 1 if interleaved, i and i + pairs
+ * if not, turned by positions[t] * inv_freq[i] and scaled by `scale`; the rest of the head is copied. positions [tokens] int32 or
+ * int64 (position_type, cernels_moe_index_type), inv_freq [pairs] fp32 or fp64 (freq_dtype); angles are formed in fp64.
+ * backward != 0 turns by the negative angles, which maps gradients of the outputs to gradients of the inputs.
+ * q_out, k_out: [tokens, heads, dim] contiguous. Limits: 2 * pairs <= dim, pairs <= 1024, (q_heads + k_heads) * dim < 2^30. */
+int cernels_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t q_heads, const void* k,
+                   int64_t k_token_stride, int64_t k_head_stride, int32_t k_heads, const void* positions, int32_t position_type,
+                   const void* inv_freq, int32_t freq_dtype, int32_t tokens, int32_t dim, int32_t pairs, int32_t interleaved,
+                   float scale, int32_t backward, int32_t dtype, void* q_out, void* k_out, hipStream_t stream);
+
+/* Paged cache. k_pages and v_pages hold `pages` pages of page_size slots (a multiple of 16) of kv_heads heads of dim elements, bf16
+ * or fp16, the last dimension contiguous; page_strides (host memory) holds k's page, slot and head stride, then v's, in elements.
+ * Sequence b's token at position p lies in slot p % page_size of page block_table[b * table_stride + p / page_size]
+ * (p / page_size < blocks). lengths [seqs] counts a sequence's tokens, the step's new ones included; its new tokens are rows
+ * q_offsets[b] .. q_offsets[b + 1] - 1 of q, k, v and out (q_offsets [seqs + 1], or NULL: tokens / seqs rows each), and the last
+ * ones of the sequence. Rows behind the last sequence are left as they were. Entries of the table outside [0, pages) have no
+ * page: nothing is written there, and their keys add nothing. Limits: seqs <= 65535, blocks * page_size < 2^31. */
+
+/* Writes k and v [tokens, kv_heads, dim] to their slots, k turned to its position as cernels_rotary does (pairs = 0: as it is);
+ * q [tokens, q_heads, dim] (nullable) is turned too, into q_out [tokens, q_heads, dim] contiguous. */
+int cernels_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t q_heads, void* q_out, const void* k,
+                         int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                         int32_t kv_heads, int32_t dim, int32_t dtype, const void* inv_freq, int32_t freq_dtype, int32_t pairs,
+                         int32_t interleaved, float scale, void* k_pages, void* v_pages, const int64_t* page_strides, int32_t pages,
+                         int32_t page_size, const int32_t* block_table, int64_t table_stride, int32_t blocks, const int32_t* lengths,
+                         const int32_t* q_offsets, int32_t seqs, int32_t tokens, hipStream_t stream);
+
+/* Attention of the step's queries q [tokens, heads, dim] over their sequences' pages, the new tokens' keys among them (append
+ * first). The query at position p sees keys j <= p, with window > 0 also j > p - window; query head h reads key head
+ * h / (heads / kv_heads); softmax of scale * q k in fp32; sinks [heads] fp32 (nullable) is one more logit of each head without a
+ * value. A row that sees nothing is 0. out [tokens, heads, dim] contiguous. max_new: the most new tokens that any sequence has, or
+ * 0 if unknown; it steers the choice of kernels only, results hold for any value. Values (V) of keys past the sequence's length
+ * or before every window of the step may hold anything.
+ * Limits: dim 64, 128 or 256; heads % kv_heads == 0; page_strides multiples of 8 and pages 16-byte aligned; scale > 0. */
+size_t cernels_paged_attention_workspace_bytes(int32_t tokens, int32_t seqs, int32_t heads, int32_t kv_heads, int32_t dim,
+                                               int32_t page_size, int32_t blocks, int32_t max_new);
+int cernels_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t heads, int32_t kv_heads,
+                            int32_t dim, int32_t dtype, const void* k_pages, const void* v_pages, const int64_t* page_strides,
+                            int32_t pages, int32_t page_size, const int32_t* block_table, int64_t table_stride, int32_t blocks,
+                            const int32_t* lengths, const int32_t* q_offsets, int32_t seqs, int32_t tokens, int32_t max_new,
+                            float scale, int32_t window, const float* sinks, void* out, void* workspace, size_t workspace_bytes,
+                            hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
