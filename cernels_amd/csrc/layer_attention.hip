@@ -13,6 +13,8 @@
 #include "layer_step.h"
 #include "moe_tile.h"
 
+#include <type_traits>
+
 namespace cmoe {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -23,23 +25,31 @@ constexpr float kNone = -__builtin_inff();
 
 struct MathBf16 {
     typedef TypeBf16 T;
-    static __device__ __forceinline__ f32x4 mma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+    static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+    static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ uint32_t pack2(float a, float b) { return pack_bf16x2(a, b); }
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) { return cvt_bf16x2(a, b); }
+    static __device__ __forceinline__ float add2(uint32_t pair, float sum) {  // sum + both values of the pair
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+    }
 };
 struct MathF16 {
     typedef TypeF16 T;
-    static __device__ __forceinline__ f32x4 mma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+    static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+    static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ uint32_t pack2(float a, float b) { return pack_f16x2(a, b); }
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) { return cvt_f16x2(a, b); }
+    static __device__ __forceinline__ float add2(uint32_t pair, float sum) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), __builtin_bit_cast(f16x2, 0x3c003c00u), sum, false);
+    }
 };
 
 // What a launch works on beside the call's own parameters.
@@ -339,12 +349,15 @@ template <class M, int D>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(AttentionParams p, AttentionPlan plan) {
     typedef typename M::T T;
     typedef typename T::raw raw;
+    typedef __attribute__((address_space(3))) const u32x4* lds_vec;
+    typedef __attribute__((address_space(3))) s16x4* lds_turned;
     constexpr int KT = TileSize<D>::kKeys, kBytes = TileSize<D>::kBytes;
-    constexpr int CH = D / 8;               // 16-byte vectors of a row
-    constexpr int kRowsPer = 64 / CH;       // rows that one copy instruction of a wave moves
-    constexpr int kCopies = KT / kRowsPer / kTileWaves;  // per wave, of each of K and V
+    constexpr int CH = D / 8, kMask = CH < 16 ? CH - 1 : 15;  // 16-byte vectors of a row; those that the banks' order permutes
+    constexpr int kRowsPer = 64 / CH;                         // rows that one copy instruction of a wave moves
+    constexpr int kRun = KT / kTileWaves, kCopies = kRun / kRowsPer;  // keys that a wave copies, all of one page
     constexpr int DS = D / 16, DT = D / 32, KU = KT / 32;
     extern __shared__ __align__(1024) unsigned char lds[];  // [2][K | V]
+    __shared__ __align__(16) uint32_t missing[2][kTileWaves];  // per wave's run of keys: without a page
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int kh = blockIdx.x % p.kv_heads, group = p.q.heads / p.kv_heads;
     TileId t;
@@ -364,36 +377,57 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(Attenti
         for (int s = 0; s < DS; ++s) q[s] = live ? load_vec<T>(src + 16 * s + 8 * h) : u32x4{};
     }
     // keys that the row, the wave's rows and the tile's rows see; positions grow with the row
-    const int cap = p.step.blocks * p.step.page_size, before = length - t.count;
+    const int page_size = p.step.page_size, cap = p.step.blocks * page_size, before = length - t.count;
     auto low = [&](int tok) { return p.window > 0 && before + tok - p.window + 1 > 0 ? before + tok - p.window + 1 : 0; };
     const int hi = live ? before + token + 1 : 0, lo = low(token);
     const int last_row = min(t.row0 + kTileRows, t.rows) - 1;
     const int w_first = min(t.row0 + 32 * wave, last_row) / group, w_last = min(t.row0 + 32 * wave + 31, last_row) / group;
     const bool idle = t.row0 + 32 * wave >= t.rows;
     const int w_hi = before + w_last + 1, w_all_hi = before + w_first + 1, w_lo = low(w_first), w_all_lo = low(w_last);
-    const int tile_lo = low(t.row0 / group) / KT * KT;
-    const int tile_hi = min(before + last_row / group + 1, cap);
+    const int tile_lo = low(t.row0 / group);
     int begin, end;
-    split_range(tile_lo, tile_hi, blockIdx.y, plan.splits, KT, 4 * KT, begin, end);
-    const int drop_lo = low(t.row0 / group);
+    split_range(tile_lo / KT * KT, min(before + last_row / group + 1, cap), blockIdx.y, plan.splits, KT, 4 * KT, begin, end);
 
-    // One tile's copies: rows past the keys that anybody sees, or without a page, come from zeros (V) or are dropped later (K).
+    // This wave's run of the next tile to copy: its page and first slot, walked along the table without a division.
+    const auto* table = (const __attribute__((address_space(4))) int32_t*)(p.step.table + t.b * p.step.table_stride);
+    int run = begin + kRun * wave, blk = run / page_size, slot = run - blk * page_size;
+    auto page_of = [&](int key, int block) {
+        const int page = key < end ? table[block] : -1;  // end is at most the table's
+        return (unsigned)page < (unsigned)p.step.pages ? page : -1;
+    };
+    int page = page_of(run, blk);
     const int crow = lane / CH, cpos = lane % CH;
-    auto copy = [&](int k0, int buf) {
-        const uint32_t base = lds_u32(lds) + buf * 2 * kBytes;
+    uint32_t koff[kCopies], voff[kCopies];  // from a copy's first row: this lane's row, and the vector that belongs at its place
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-            const int r0 = (wave * kCopies + i) * kRowsPer;  // of the tile, the same in all lanes; its rows lie in one page
-            const int key = k0 + r0, blk = key / p.step.page_size, slot = key - blk * p.step.page_size;
-            const int page = key < end ? step_page(p.step, t.b, blk) : -1;
-            const long long at = page < 0 ? 0 : page;
-            const int r = r0 + crow;
-            const char* kp = kbase + 2 * (at * p.k.page + (slot + crow) * p.k.slot) + 16 * (cpos ^ (r & (CH - 1) & 15));
-            dma16(kp, base + r0 * D * 2);
-            const char* vp = vbase + 2 * (at * p.v.page + (slot + crow) * p.v.slot) + 16 * (cpos ^ (2 * r & (CH - 1) & 15));
-            const bool zero = page < 0 || k0 + r >= end || k0 + r < drop_lo;
-            dma16(zero ? reinterpret_cast<const char*>(kZeros) : vp, base + kBytes + r0 * D * 2);
+    for (int i = 0; i < kCopies; ++i) {
+        const int r = wave * kRun + i * kRowsPer + crow;
+        koff[i] = (uint32_t)(2 * crow * p.k.slot) + 16 * (cpos ^ (r & kMask));
+        voff[i] = (uint32_t)(2 * crow * p.v.slot) + 16 * (cpos ^ (2 * r & kMask));
+    }
+    auto copy = [&](int buf) {
+        const uint32_t dst = lds_u32(lds) + buf * 2 * kBytes + wave * kRun * D * 2;
+        const long long at = page < 0 ? 0 : page;  // keys without a page are read from page 0 and dropped below
+        const char* kp = kbase + 2 * (at * p.k.page + slot * p.k.slot);
+        const char* vp = vbase + 2 * (at * p.v.page + slot * p.v.slot);
+        const bool plain = page >= 0 && run >= tile_lo && run + kRun <= end;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) dma16_at(kp + 2 * i * kRowsPer * p.k.slot, koff[i], dst + i * 1024);
+        if (plain) {
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) dma16_at(vp + 2 * i * kRowsPer * p.v.slot, voff[i], dst + kBytes + i * 1024);
+        } else {  // values that nobody sees may be anything, and 0 times anything is not always 0
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                const int key = run + i * kRowsPer + crow;
+                const bool zero = page < 0 || key >= end || key < tile_lo;
+                dma16(zero ? reinterpret_cast<const char*>(kZeros) : vp + 2 * i * kRowsPer * p.v.slot + voff[i], dst + kBytes + i * 1024);
+            }
         }
+        if (lane == 0) missing[buf][wave] = page < 0;
+        run += KT;
+        slot += KT;
+        while (slot >= page_size) slot -= page_size, ++blk;
+        page = page_of(run, blk);
     };
 
     float m = kNone, l = 0.0f;
@@ -402,43 +436,39 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(Attenti
     for (int j = 0; j < DT; ++j)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[j][i] = 0.0f;
+    // Where this lane reads its operands: K's row `col`, vector 2 d + h; V's 4 keys x 16 columns for each 16 lanes, of which lane n
+    // addresses 4 columns of key n / 4 and gets column n.
+    uint32_t kaddr[DS], vaddr[DT];
+#pragma unroll
+    for (int d = 0; d < DS; ++d) kaddr[d] = lds_u32(lds) + col * D * 2 + 16 * ((2 * d + h) ^ (col & kMask));
+#pragma unroll
+    for (int j = 0; j < DT; ++j) {
+        const int r = 4 * h + (lane & 15) / 4, chunk = 4 * j + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        vaddr[j] = lds_u32(lds) + kBytes + r * D * 2 + 16 * (chunk ^ (2 * r & kMask)) + 8 * (lane & 1);
+    }
 
-    int buf = 0;
-    if (begin < end) copy(begin, 0);
-    for (int k0 = begin; k0 < end; k0 += KT, buf ^= 1) {
-        wait_vmcnt<0>();
-        __syncthreads();
-        if (k0 + KT < end) copy(k0 + KT, buf ^ 1);
-        if (idle || k0 >= w_hi || k0 + KT <= w_lo) continue;
-        const unsigned char* kt = lds + buf * 2 * kBytes;
-        const uint32_t vt = lds_u32(kt) + kBytes;
+    auto work = [&](int k0, auto which) {
+        constexpr int kBase = decltype(which)::value * 2 * kBytes;
         f32x16 s[KU];
 #pragma unroll
-        for (int u = 0; u < KU; ++u) {
+        for (int u = 0; u < KU; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
-            const int r = 32 * u + col;
 #pragma unroll
-            for (int d = 0; d < DS; ++d) {
-                const u32x4 a = *reinterpret_cast<const u32x4*>(kt + r * D * 2 + 16 * ((2 * d + h) ^ (r & (CH - 1) & 15)));
-                s[u] = M::mma32(a, q[d], s[u]);
-            }
-        }
-        bool whole = k0 >= w_all_lo && k0 + KT <= w_all_hi && k0 + KT <= end;
-        uint32_t pages_bad = 0;  // bit r / 16: the 16 keys have no page
+        for (int d = 0; d < DS; ++d)
 #pragma unroll
-        for (int r = 0; r < KT; r += 16) {
-            const int blk = (k0 + r) / p.step.page_size;
-            if (k0 + r < end && step_page(p.step, t.b, blk) < 0) pages_bad |= 1u << (r / 16);
-        }
-        if (pages_bad) whole = false;
+            for (int u = 0; u < KU; ++u) s[u] = M::mma32(*(lds_vec)(kaddr[d] + kBase + u * 32 * D * 2), q[d], s[u]);
+        uint32_t gone[kTileWaves], any = 0;
+#pragma unroll
+        for (int w = 0; w < kTileWaves; ++w) any |= gone[w] = missing[decltype(which)::value][w];
+        const bool whole = k0 >= w_all_lo && k0 + KT <= w_all_hi && k0 + KT <= end && !__builtin_amdgcn_readfirstlane(any);
         if (!whole) {
 #pragma unroll
             for (int u = 0; u < KU; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int r = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3), key = k0 + r;
-                    const bool sees = key < hi && key >= lo && key < end && !(pages_bad >> (r / 16) & 1);
+                    const bool sees = key < hi && key >= lo && key < end && !gone[(32 * u + 8 * (i >> 2)) / kRun];
                     s[u][i] = sees ? s[u][i] : kNone;
                 }
         }
@@ -463,27 +493,38 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(Attenti
             for (int k = 0; k < 2; ++k) {
                 float e[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * k + i], c, -sub));
-                    l += e[i];
-                }
+                for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * k + i], c, -sub));
+                // Rounded to the values' type for the product. The sum takes the rounded ones too: what rounding does to a row's
+                // weights as a whole then cancels.
                 const u32x4 pr{M::pack2(e[0], e[1]), M::pack2(e[2], e[3]), M::pack2(e[4], e[5]), M::pack2(e[6], e[7])};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) l = M::add2(pr[i], l);
 #pragma unroll
                 for (int j = 0; j < DT; ++j) {
                     u32x4 a;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        // 4 keys x 16 columns for each 16 lanes: lane n of them addresses 4 columns of key n / 4 and gets column n
-                        const int r = 32 * u + 16 * k + 8 * i + 4 * h + (lane & 15) / 4;
-                        const int chunk = 4 * j + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                        const uint32_t at = vt + r * D * 2 + 16 * (chunk ^ (2 * r & (CH - 1) & 15)) + 8 * (lane & 1);
-                        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+                        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_turned)(vaddr[j] + kBase + (32 * u + 16 * k + 8 * i) * D * 2));
                         const u32x2 w = __builtin_bit_cast(u32x2, v);
                         a[2 * i] = w[0], a[2 * i + 1] = w[1];
                     }
                     o[j] = M::mma32(a, pr, o[j]);
                 }
             }
+    };
+    // One tile: its copies have landed, the next one's are sent, and no wave is still reading what they replace.
+    auto step = [&](int k0, auto which) {
+        wait_vmcnt<0>();
+        __syncthreads();
+        if (k0 + KT < end) copy(1 - decltype(which)::value);
+        if (!idle && k0 < w_hi && k0 + KT > w_lo) work(k0, which);
+    };
+    wait_all_loads();  // the queries: a wait for them inside the loop would be one for the copies too
+    if (begin < end) copy(0);
+    for (int k0 = begin; k0 < end; k0 += 2 * KT) {
+        step(k0, std::integral_constant<int, 0>{});
+        if (k0 + KT >= end) break;
+        step(k0 + KT, std::integral_constant<int, 1>{});
     }
     {
         uint32_t a = __float_as_uint(l), b = a;

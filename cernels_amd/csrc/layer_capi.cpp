@@ -36,6 +36,8 @@ int step_checks(const cmoe::StepView& s) {
 bool pages_ok(const cmoe::PagesView& v) {
     return aligned(v.p, 16) && v.page % 8 == 0 && v.slot % 8 == 0 && v.head % 8 == 0 && v.page >= 0 && v.slot >= 0 && v.head >= 0;
 }
+// A run of 16 slots is reached by 32-bit offsets.
+bool runs_ok(const cmoe::PagesView& v) { return v.slot < (1LL << 26); }
 
 cmoe::StepView step_of(const int32_t* table, int64_t table_stride, const int32_t* lengths, const int32_t* offsets, int32_t seqs,
                        int32_t tokens, int32_t pages, int32_t page_size, int32_t blocks) {
@@ -178,6 +180,7 @@ int cernels_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
     p.sinks = sinks, p.out = out, p.scale = scale, p.ws = static_cast<float*>(workspace);
     if (!aligned(q, 2) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(sinks, 4) || !pages_ok(p.k) || !pages_ok(p.v))
         return CERNELS_MOE_MISALIGNED;
+    if (!runs_ok(p.k) || !runs_ok(p.v)) return CERNELS_MOE_UNSUPPORTED_SHAPE;
     if (workspace_bytes < cmoe::attention_workspace_bytes(p)) return CERNELS_MOE_WORKSPACE_TOO_SMALL;
     return hip_status(cmoe::launch_attention(p, stream));
 }

@@ -11,6 +11,18 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));  // a vector at any element's address: global accesses
 typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));  // of gfx950 need no alignment beyond the element's
 
+// Two fp32 values as two 16-bit ones, rounded to nearest even, in one conversion (low half = a).
+__device__ __forceinline__ uint32_t cvt_bf16x2(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+__device__ __forceinline__ uint32_t cvt_f16x2(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+}
+
 struct TypeBf16 {
     typedef uint16_t raw;
     typedef u32x4_a2 loose;
@@ -22,7 +34,7 @@ struct TypeBf16 {
         for (int i = 0; i < 4; ++i) f[2 * i] = bf16_lo(r[i]), f[2 * i + 1] = bf16_hi(r[i]);
     }
     static __device__ __forceinline__ u32x4 pack(const float* f) {
-        return u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+        return u32x4{cvt_bf16x2(f[0], f[1]), cvt_bf16x2(f[2], f[3]), cvt_bf16x2(f[4], f[5]), cvt_bf16x2(f[6], f[7])};
     }
 };
 
@@ -38,7 +50,7 @@ struct TypeF16 {
         for (int i = 0; i < 8; ++i) f[i] = (float)h[i];
     }
     static __device__ __forceinline__ u32x4 pack(const float* f) {
-        return u32x4{pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7])};
+        return u32x4{cvt_f16x2(f[0], f[1]), cvt_f16x2(f[2], f[3]), cvt_f16x2(f[4], f[5]), cvt_f16x2(f[6], f[7])};
     }
 };
 

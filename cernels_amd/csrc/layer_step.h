@@ -37,4 +37,10 @@ __device__ __forceinline__ int step_page(const StepView& s, int b, int blk) {
     return (unsigned)page < (unsigned)s.pages ? page : -1;
 }
 
+// One copy instruction of a wave, 16 bytes per lane, from a uniform base and a lane's own offset into 1 KB of LDS; waits and
+// ordering are the caller's, as for dma16 (moe_tile.h).
+__device__ __forceinline__ void dma16_at(const void* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "memory", "m0");
+}
+
 }  // namespace cmoe

@@ -331,7 +331,8 @@ int cernels_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_s
  * value. A row that sees nothing is 0. out [tokens, heads, dim] contiguous. max_new: the most new tokens that any sequence has, or
  * 0 if unknown; it steers the choice of kernels only, results hold for any value. Values (V) of keys past the sequence's length
  * or before every window of the step may hold anything.
- * Limits: dim 64, 128 or 256; heads % kv_heads == 0; page_strides multiples of 8 and pages 16-byte aligned; scale > 0. */
+ * Limits: dim 64, 128 or 256; heads % kv_heads == 0; page_strides multiples of 8, the slots' under 2^26, pages 16-byte
+ * aligned; scale > 0. */
 size_t cernels_paged_attention_workspace_bytes(int32_t tokens, int32_t seqs, int32_t heads, int32_t kv_heads, int32_t dim,
                                                int32_t page_size, int32_t blocks, int32_t max_new);
 int cernels_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t heads, int32_t kv_heads,
