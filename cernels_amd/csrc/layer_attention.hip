@@ -336,8 +336,7 @@ __device__ __forceinline__ bool find_tile(const AttentionParams& p, const Attent
             t.first = __builtin_amdgcn_readlane(first, l);
             t.count = __builtin_amdgcn_readlane(count, l);
             t.rows = __builtin_amdgcn_readlane(rows, l);
-            const int before = __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(tiles, l);
-            t.row0 = (i - before) * kTileRows;
+            t.row0 = (__builtin_amdgcn_readlane(sum, l) - 1 - i) * kTileRows;  // the last tile first: it sees the most keys
             return true;
         }
         i -= __builtin_amdgcn_readlane(sum, 63);
@@ -614,7 +613,7 @@ static Forms attention_forms(const AttentionParams& p) {
     const long long seqs = p.step.seqs < rows / (kFewMost + 1) ? p.step.seqs : rows / (kFewMost + 1);
     f.tiles = f.tile ? (int)((rows + kTileRows - 1) / kTileRows + seqs) : 0;
     const long long groups = f.tile ? (long long)f.tiles * p.kv_heads : (long long)p.step.seqs * p.kv_heads;
-    const long long want = (f.tile ? 512 : f.most > 16 ? 2048 : 4096) / groups;
+    const long long want = ((f.tile ? 512 : f.most > 16 ? 2048 : 4096) + groups / 2) / groups;
     const long long useful = (keys + 255) / 256;
     const long long n = want < useful ? want : useful;
     f.splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
