@@ -345,7 +345,7 @@ __device__ __forceinline__ bool find_tile(const AttentionParams& p, const Attent
 }
 
 template <class M, int D>
-__global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(AttentionParams p, AttentionPlan plan) {
+__global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile_kernel(AttentionParams p, AttentionPlan plan) {
     typedef typename M::T T;
     typedef typename T::raw raw;
     typedef __attribute__((address_space(3))) const u32x4* lds_vec;
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(Attenti
     constexpr int kRun = KT / kTileWaves, kCopies = kRun / kRowsPer;  // keys that a wave copies, all of one page
     constexpr int DS = D / 16, DT = D / 32, KU = KT / 32;
     extern __shared__ __align__(1024) unsigned char lds[];  // [2][K | V]
-    __shared__ __align__(16) uint32_t missing[2][kTileWaves];  // per wave's run of keys: without a page
+    __shared__ __align__(16) uint32_t missing[4][kTileWaves];  // per tile and wave's run of keys: without a page
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int kh = blockIdx.x % p.kv_heads, group = p.q.heads / p.kv_heads;
     TileId t;
@@ -377,7 +377,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(Attenti
     }
     // keys that the row, the wave's rows and the tile's rows see; positions grow with the row
     const int page_size = p.step.page_size, cap = p.step.blocks * page_size, before = length - t.count;
-    auto low = [&](int tok) { return p.window > 0 && before + tok - p.window + 1 > 0 ? before + tok - p.window + 1 : 0; };
+    auto low = [&](int tok) __attribute__((always_inline)) { return p.window > 0 && before + tok - p.window + 1 > 0 ? before + tok - p.window + 1 : 0; };
     const int hi = live ? before + token + 1 : 0, lo = low(token);
     const int last_row = min(t.row0 + kTileRows, t.rows) - 1;
     const int w_first = min(t.row0 + 32 * wave, last_row) / group, w_last = min(t.row0 + 32 * wave + 31, last_row) / group;
@@ -387,14 +387,22 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(Attenti
     int begin, end;
     split_range(tile_lo / KT * KT, min(before + last_row / group + 1, cap), blockIdx.y, plan.splits, KT, 4 * KT, begin, end);
 
-    // This wave's run of the next tile to copy: its page and first slot, walked along the table without a division.
+    // This wave's run of the next tile to copy: its page and first slot, walked along the table without a division. Keys are sent one
+    // tile ahead of the values, so the values' run is the one that the keys had before.
+    struct Run {
+        int key, blk, slot, page;
+    };
     const auto* table = (const __attribute__((address_space(4))) int32_t*)(p.step.table + t.b * p.step.table_stride);
-    int run = begin + kRun * wave, blk = run / page_size, slot = run - blk * page_size;
-    auto page_of = [&](int key, int block) {
+    auto page_of = [&](int key, int block) __attribute__((always_inline)) {
         const int page = key < end ? table[block] : -1;  // end is at most the table's
         return (unsigned)page < (unsigned)p.step.pages ? page : -1;
     };
-    int page = page_of(run, blk);
+    Run kr, vr;
+    kr.key = begin + kRun * wave;
+    kr.blk = kr.key / page_size;
+    kr.slot = kr.key - kr.blk * page_size;
+    kr.page = page_of(kr.key, kr.blk);
+    vr = kr;
     const int crow = lane / CH, cpos = lane % CH;
     uint32_t koff[kCopies], voff[kCopies];  // from a copy's first row: this lane's row, and the vector that belongs at its place
 #pragma unroll
@@ -403,30 +411,34 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(Attenti
         koff[i] = (uint32_t)(2 * crow * p.k.slot) + 16 * (cpos ^ (r & kMask));
         voff[i] = (uint32_t)(2 * crow * p.v.slot) + 16 * (cpos ^ (2 * r & kMask));
     }
-    auto copy = [&](int buf) {
-        const uint32_t dst = lds_u32(lds) + buf * 2 * kBytes + wave * kRun * D * 2;
-        const long long at = page < 0 ? 0 : page;  // keys without a page are read from page 0 and dropped below
-        const char* kp = kbase + 2 * (at * p.k.page + slot * p.k.slot);
-        const char* vp = vbase + 2 * (at * p.v.page + slot * p.v.slot);
-        const bool plain = page >= 0 && run >= tile_lo && run + kRun <= end;
+    const uint32_t mine = lds_u32(lds) + wave * kRun * D * 2;
+    auto copy_keys = [&](int tile) __attribute__((always_inline)) {
+        const uint32_t dst = mine + (tile & 1) * 2 * kBytes;
+        const long long at = kr.page < 0 ? 0 : kr.page;  // keys without a page are read from page 0 and dropped below
+        const char* kp = kbase + 2 * (at * p.k.page + kr.slot * p.k.slot);
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) dma16_at(kp + 2 * i * kRowsPer * p.k.slot, koff[i], dst + i * 1024);
-        if (plain) {
+        if (lane == 0) missing[tile & 3][wave] = kr.page < 0;
+        kr.key += KT;
+        kr.slot += KT;
+        while (kr.slot >= page_size) kr.slot -= page_size, ++kr.blk;
+        kr.page = page_of(kr.key, kr.blk);
+    };
+    auto copy_values = [&](int tile, const Run& r) __attribute__((always_inline)) {
+        const uint32_t dst = mine + (tile & 1) * 2 * kBytes + kBytes;
+        const long long at = r.page < 0 ? 0 : r.page;
+        const char* vp = vbase + 2 * (at * p.v.page + r.slot * p.v.slot);
+        if (r.page >= 0 && r.key >= tile_lo && r.key + kRun <= end) {
 #pragma unroll
-            for (int i = 0; i < kCopies; ++i) dma16_at(vp + 2 * i * kRowsPer * p.v.slot, voff[i], dst + kBytes + i * 1024);
+            for (int i = 0; i < kCopies; ++i) dma16_at(vp + 2 * i * kRowsPer * p.v.slot, voff[i], dst + i * 1024);
         } else {  // values that nobody sees may be anything, and 0 times anything is not always 0
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) {
-                const int key = run + i * kRowsPer + crow;
-                const bool zero = page < 0 || key >= end || key < tile_lo;
-                dma16(zero ? reinterpret_cast<const char*>(kZeros) : vp + 2 * i * kRowsPer * p.v.slot + voff[i], dst + kBytes + i * 1024);
+                const int key = r.key + i * kRowsPer + crow;
+                const bool zero = r.page < 0 || key >= end || key < tile_lo;
+                dma16(zero ? reinterpret_cast<const char*>(kZeros) : vp + 2 * i * kRowsPer * p.v.slot + voff[i], dst + i * 1024);
             }
         }
-        if (lane == 0) missing[buf][wave] = page < 0;
-        run += KT;
-        slot += KT;
-        while (slot >= page_size) slot -= page_size, ++blk;
-        page = page_of(run, blk);
     };
 
     float m = kNone, l = 0.0f;
@@ -446,20 +458,26 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(Attenti
         vaddr[j] = lds_u32(lds) + kBytes + r * D * 2 + 16 * (chunk ^ (2 * r & kMask)) + 8 * (lane & 1);
     }
 
-    auto work = [&](int k0, auto which) {
+    f32x16 s[KU];
+    auto scores = [&](auto which) __attribute__((always_inline)) {  // of the tile whose keys lie in buffer `which`
         constexpr int kBase = decltype(which)::value * 2 * kBytes;
-        f32x16 s[KU];
+        f32x16 r[KU];
 #pragma unroll
         for (int u = 0; u < KU; ++u)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) r[u][i] = 0.0f;
 #pragma unroll
         for (int d = 0; d < DS; ++d)
 #pragma unroll
-            for (int u = 0; u < KU; ++u) s[u] = M::mma32(*(lds_vec)(kaddr[d] + kBase + u * 32 * D * 2), q[d], s[u]);
+            for (int u = 0; u < KU; ++u) r[u] = M::mma32(*(lds_vec)(kaddr[d] + kBase + u * 32 * D * 2), q[d], r[u]);
+#pragma unroll
+        for (int u = 0; u < KU; ++u) s[u] = r[u];
+    };
+    // The running maximum over s, the scores of the tile at k0; hidden ones become -inf.
+    auto raise = [&](int k0, int tile) __attribute__((always_inline)) {
         uint32_t gone[kTileWaves], any = 0;
 #pragma unroll
-        for (int w = 0; w < kTileWaves; ++w) any |= gone[w] = missing[decltype(which)::value][w];
+        for (int w = 0; w < kTileWaves; ++w) any |= gone[w] = missing[tile & 3][w];
         const bool whole = k0 >= w_all_lo && k0 + KT <= w_all_hi && k0 + KT <= end && !__builtin_amdgcn_readfirstlane(any);
         if (!whole) {
 #pragma unroll
@@ -467,7 +485,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(Attenti
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int r = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3), key = k0 + r;
-                    const bool sees = key < hi && key >= lo && key < end && !gone[(32 * u + 8 * (i >> 2)) / kRun];
+                    const bool sees = (key < hi) & (key >= lo) & (key < end) & (gone[(32 * u + 8 * (i >> 2)) / kRun] == 0);
                     s[u][i] = sees ? s[u][i] : kNone;
                 }
         }
@@ -485,14 +503,22 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(Attenti
 #pragma unroll
             for (int j = 0; j < DT; ++j) o[j] *= f;
         }
+    };
+    // The probabilities of s and their product with the values in buffer `which`; between them the next tile's scores.
+    auto weigh = [&](auto which, auto more) __attribute__((always_inline)) {
+        constexpr int kBase = decltype(which)::value * 2 * kBytes;
         const float sub = m == kNone ? 0.0f : m;
+        f32x16 t[KU];
+#pragma unroll
+        for (int u = 0; u < KU; ++u) t[u] = s[u];
+        if constexpr (decltype(more)::value) scores(std::integral_constant<int, 1 - decltype(which)::value>{});
 #pragma unroll
         for (int u = 0; u < KU; ++u)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 float e[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * k + i], c, -sub));
+                for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[u][8 * k + i], c, -sub));
                 // Rounded to the values' type for the product. The sum takes the rounded ones too: what rounding does to a row's
                 // weights as a whole then cancels.
                 const u32x4 pr{M::pack2(e[0], e[1]), M::pack2(e[2], e[3]), M::pack2(e[4], e[5]), M::pack2(e[6], e[7])};
@@ -511,19 +537,37 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void attend_tile_kernel(Attenti
                 }
             }
     };
-    // One tile: its copies have landed, the next one's are sent, and no wave is still reading what they replace.
-    auto step = [&](int k0, auto which) {
+    // One tile. What was sent a tile ago has landed (its values, the next one's keys); the keys of the tile after that and the next
+    // values are sent into the buffers that no wave reads any more.
+    auto step = [&](int k0, int tile, auto which) __attribute__((always_inline)) {
+        const bool more = k0 + KT < end;
         wait_vmcnt<0>();
         __syncthreads();
-        if (k0 + KT < end) copy(1 - decltype(which)::value);
-        if (!idle && k0 < w_hi && k0 + KT > w_lo) work(k0, which);
+        if (more) {
+            const Run next = kr;
+            if (k0 + 2 * KT < end) copy_keys(tile + 2);
+            copy_values(tile + 1, vr);
+            vr = next;
+        }
+        if (idle) return;
+        raise(k0, tile);
+        if (more) weigh(which, std::true_type{});
+        else weigh(which, std::false_type{});
     };
     wait_all_loads();  // the queries: a wait for them inside the loop would be one for the copies too
-    if (begin < end) copy(0);
-    for (int k0 = begin; k0 < end; k0 += 2 * KT) {
-        step(k0, std::integral_constant<int, 0>{});
+    if (begin < end) {
+        copy_keys(0);
+        copy_values(0, vr);
+        vr = kr;
+        wait_vmcnt<0>();
+        __syncthreads();
+        if (begin + KT < end) copy_keys(1);
+        if (!idle) scores(std::integral_constant<int, 0>{});
+    }
+    for (int k0 = begin, tile = 0; k0 < end; k0 += 2 * KT, tile += 2) {
+        step(k0, tile, std::integral_constant<int, 0>{});
         if (k0 + KT >= end) break;
-        step(k0 + KT, std::integral_constant<int, 1>{});
+        step(k0 + KT, tile + 1, std::integral_constant<int, 1>{});
     }
     {
         uint32_t a = __float_as_uint(l), b = a;
