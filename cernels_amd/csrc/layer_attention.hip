@@ -28,6 +28,9 @@ struct MathBf16 {
     static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f32x4 mma16_short(s16x4 a, u32x2 b, f32x4 c) {  // 16 x 16 x 16
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+    }
     static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
@@ -41,6 +44,10 @@ struct MathF16 {
     typedef TypeF16 T;
     static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 mma16_short(s16x4 a, u32x2 b, f32x4 c) {
+        typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -81,33 +88,61 @@ __device__ __forceinline__ float row_scale(const AttentionParams& p, int head, f
     return l > 0.0f || l != l ? 1.0f / l : 0.0f;  // a row that sees nothing is 0
 }
 
+__device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
+
 // ---- few rows: single tokens and short chunks ---------------------------------------------------------------------------------
-// Bound by the stream of keys and values. A wave takes 32 keys at a time straight from memory into the operand registers of the
-// 16 x 16 x 32 products, with no LDS between: K's rows as they lie (16 rows x 64 contiguous bytes an instruction), V's rows whole
-// (contiguous), turned by permutes of 16-bit halves within the lane. Four waves of a workgroup share out its keys.
+// Bound by the stream of keys and values. The four waves of a workgroup share out its keys, and each runs alone: 16 keys at a time
+// come through a ring of two stages of its own in LDS, sent there without passing through registers, so that 16 to 32 KB per wave
+// are on their way at any time however few registers the products leave. Keys are read as operands as they lie, values turned
+// (ds_read_b64_tr_b16: 4 keys of one column per lane).
 constexpr int kFewWaves = 4;
-constexpr int kFewKeys = 32;
+constexpr int kFewKeys = 16;
+constexpr int kFewLeast = 256;  // keys of a split
 
 template <class M, int D, int NT>
 __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionParams p, AttentionPlan plan) {
     typedef typename M::T T;
     typedef typename T::raw raw;
-    constexpr int DS = D / 32;      // steps of the first product
-    constexpr int DJ = D / 16;      // 16-row tiles of the second one's result
-    constexpr int VC = D / 16 / 8 ? D / 128 : 0;  // 16-byte vectors of a V row per lane (0: one 8-byte vector)
-    __shared__ float lds_o[kFewWaves][16 * D];
+    typedef __attribute__((address_space(3))) const u32x4* lds_vec;
+    typedef __attribute__((address_space(3))) s16x4* lds_turned;
+    constexpr int DS = D / 32;                                // steps of the first product
+    constexpr int DJ = D / 16;                                // 16-row tiles of the second one's result
+    constexpr int CH = D / 8, kMask = CH < 16 ? CH - 1 : 15;  // 16-byte vectors of a row; those that the banks' order permutes
+    constexpr int kRowsPer = 64 / CH, kCopies = kFewKeys / kRowsPer;
+    constexpr int kBytes = kFewKeys * D * 2, kWaveBytes = 4 * kBytes;  // a stage's keys; a wave's ring: [2][K | V]
+    extern __shared__ __align__(1024) unsigned char lds[];             // the rings; afterwards the waves' results
     __shared__ float2 lds_ml[kFewWaves][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    float* lds_o = reinterpret_cast<float*>(lds);  // [wave][16 * D]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int b = blockIdx.z, kh = blockIdx.y;
     const int group = p.q.heads / p.kv_heads;
     int first, count;
     step_tokens(p.step, b, first, count);
     const int rows = count * group;
     if (rows == 0 || (plan.few_rows > 0 && rows > plan.few_rows)) return;
-    const int length = p.step.lengths[b];
+    const int length = p.step.lengths[b], page_size = p.step.page_size;
     const char* kbase = static_cast<const char*>(p.k.p) + 2 * kh * p.k.head;
     const char* vbase = static_cast<const char*>(p.v.p) + 2 * kh * p.v.head;
+    const auto* table = (const __attribute__((address_space(4))) int32_t*)(p.step.table + b * p.step.table_stride);
     const float c = p.scale * kLog2e;
+    // from a copy's first row: this lane's row, and the vector that belongs at its place
+    const int crow = lane / CH, cpos = lane % CH;
+    uint32_t koff[kCopies], voff[kCopies];
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+        const int r = i * kRowsPer + crow;
+        koff[i] = (uint32_t)(2 * crow * p.k.slot) + 16 * (cpos ^ (r & kMask));
+        voff[i] = (uint32_t)(2 * crow * p.v.slot) + 16 * (cpos ^ (2 * r & kMask));
+    }
+    const uint32_t ring = lds_u32(lds) + wave * kWaveBytes;
+    uint32_t kaddr[DS], vaddr[DJ];
+#pragma unroll
+    for (int d = 0; d < DS; ++d) kaddr[d] = ring + col * D * 2 + 16 * ((4 * d + g) ^ (col & kMask));
+#pragma unroll
+    for (int j = 0; j < DJ; ++j) {
+        const int r = 4 * g + col / 4, chunk = 2 * j + ((lane & 3) >> 1);
+        vaddr[j] = ring + kBytes + r * D * 2 + 16 * (chunk ^ (2 * r & kMask)) + 8 * (lane & 1);
+    }
 
     for (int r0 = 0; r0 < rows; r0 += 16 * NT) {
         // rows r0 .. r0 + 16 NT - 1: this lane's columns, their queries and the keys that they see
@@ -138,12 +173,49 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
             all_hi = min(all_hi, __shfl_xor(all_hi, o));
             all_lo = max(all_lo, __shfl_xor(all_lo, o));
         }
-        most_hi = __builtin_amdgcn_readfirstlane(min(most_hi, p.step.blocks * p.step.page_size));
+        most_hi = __builtin_amdgcn_readfirstlane(min(most_hi, p.step.blocks * page_size));
         least_lo = __builtin_amdgcn_readfirstlane(least_lo);
         all_hi = __builtin_amdgcn_readfirstlane(all_hi);
         all_lo = __builtin_amdgcn_readfirstlane(all_lo);
         int begin, end;
-        split_range(least_lo & ~(kFewKeys - 1), most_hi, blockIdx.x, plan.splits, kFewKeys * kFewWaves, 2 * kFewKeys * kFewWaves, begin, end);
+        split_range(least_lo & ~(kFewKeys - 1), most_hi, blockIdx.x, plan.splits, kFewKeys * kFewWaves, kFewLeast, begin, end);
+        // this wave's quarter of them; a stage lies inside one page (pages hold a multiple of 16 slots), and the pages are walked along
+        // the table without a division
+        const int quarter = (end - begin + kFewKeys * kFewWaves - 1) / (kFewKeys * kFewWaves) * kFewKeys;
+        const int w_begin = min(begin + wave * quarter, end), w_end = min(w_begin + quarter, end);
+        struct Run {
+            int key, blk, slot, page;
+        };
+        auto look = [&](Run& r) __attribute__((always_inline)) {
+            const int page = r.key < w_end ? table[r.blk] : -1;  // w_end is at most the table's
+            r.page = (unsigned)page < (unsigned)p.step.pages ? page : -1;
+        };
+        auto walk = [&](Run& r) __attribute__((always_inline)) {
+            r.key += kFewKeys;
+            r.slot += kFewKeys;
+            if (r.slot >= page_size) r.slot -= page_size, ++r.blk;
+            look(r);
+        };
+        auto copy_keys = [&](const Run& r, int stage) __attribute__((always_inline)) {
+            const char* kp = kbase + 2 * ((long long)max(r.page, 0) * p.k.page + r.slot * p.k.slot);  // without a page: page 0, dropped below
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) dma16_at(kp + 2 * i * kRowsPer * p.k.slot, koff[i], ring + stage * 2 * kBytes + i * 1024);
+        };
+        auto copy_values = [&](const Run& r, int stage) __attribute__((always_inline)) {
+            const char* vp = vbase + 2 * ((long long)max(r.page, 0) * p.v.page + r.slot * p.v.slot);
+            const uint32_t dst = ring + stage * 2 * kBytes + kBytes;
+            if (r.page >= 0 && r.key >= least_lo && r.key + kFewKeys <= w_end) {
+#pragma unroll
+                for (int i = 0; i < kCopies; ++i) dma16_at(vp + 2 * i * kRowsPer * p.v.slot, voff[i], dst + i * 1024);
+            } else {  // values that nobody sees may be anything, and 0 times anything is not always 0
+#pragma unroll
+                for (int i = 0; i < kCopies; ++i) {
+                    const int key = r.key + i * kRowsPer + crow;
+                    const bool zero = r.page < 0 || key >= w_end || key < least_lo;
+                    dma16(zero ? reinterpret_cast<const char*>(kZeros) : vp + 2 * i * kRowsPer * p.v.slot + voff[i], dst + i * 1024);
+                }
+            }
+        };
 
         float m[NT], l[NT];
         f32x4 o[NT][DJ];
@@ -154,69 +226,36 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
 #pragma unroll
             for (int j = 0; j < DJ; ++j) o[n][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        for (int k0 = begin + kFewKeys * wave; k0 < end; k0 += kFewKeys * kFewWaves) {
-            // two runs of 16 keys, each inside one page (pages hold a multiple of 16 keys)
-            u32x4 kr[2][DS];
-            uint32_t vr[8][D / 32];
-            bool bad[2];
+        // One stage: 16 keys from k0, `left` keys to come with them. K of the stage after next is sent once this stage's is read, V
+        // likewise; a wait leaves in flight what was sent after what it waits for.
+        auto step = [&](int k0, int left, bool bad, const Run& next, auto which) __attribute__((always_inline)) {
+            constexpr int kBase = decltype(which)::value * 2 * kBytes;
+            if (left > kFewKeys) wait_vmcnt<3 * kCopies>();
+            else wait_vmcnt<kCopies>();
+            f32x4 s[NT];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int key = k0 + 16 * u, blk = key / p.step.page_size, slot = key - blk * p.step.page_size;
-                const int page = key < end ? step_page(p.step, b, blk) : -1;
-                bad[u] = page < 0;
-                const long long at = page < 0 ? 0 : page;  // a key that nobody sees is read from page 0 and dropped below
-                const char* kp = kbase + 2 * (at * p.k.page + (slot + col) * p.k.slot);
+            for (int n = 0; n < NT; ++n) s[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int s = 0; s < DS; ++s) kr[u][s] = *reinterpret_cast<const u32x4*>(kp + 16 * (g + 4 * s));
-                const char* vp = vbase + 2 * (at * p.v.page + (slot + 4 * g) * p.v.slot);
+            for (int d = 0; d < DS; ++d) {
+                const u32x4 a = *(lds_vec)(kaddr[d] + kBase);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const char* row = vp + 2 * i * p.v.slot;
-                    if constexpr (VC == 0) {
-                        const u32x2 t = *reinterpret_cast<const u32x2*>(row + 8 * col);
-                        vr[4 * u + i][0] = t[0], vr[4 * u + i][1] = t[1];
-                    } else {
-#pragma unroll
-                        for (int v = 0; v < VC; ++v) {
-                            const u32x4 t = *reinterpret_cast<const u32x4*>(row + 16 * col + 256 * v);
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) vr[4 * u + i][4 * v + w] = t[w];
-                        }
-                    }
-                }
+                for (int n = 0; n < NT; ++n) s[n] = M::mma16(a, q[n][d], s[n]);
             }
-            const bool whole = !bad[0] && !bad[1] && k0 >= all_lo && k0 + kFewKeys <= all_hi && k0 + kFewKeys <= end;
-            if (!whole) {  // values of keys outside the sequence may be anything, and 0 times anything is not always 0
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int key = k0 + 16 * (i >> 2) + 4 * g + (i & 3);
-                    const bool drop = bad[i >> 2] || key >= end || key < least_lo;
-#pragma unroll
-                    for (int w = 0; w < D / 32; ++w) vr[i][w] = drop ? 0u : vr[i][w];
-                }
-            }
-            u32x4 pr[NT];
+            const bool sent = left > 2 * kFewKeys;
+            if (sent) copy_keys(next, decltype(which)::value);
+            const bool whole = !bad && k0 >= all_lo && k0 + kFewKeys <= all_hi && left >= kFewKeys;
+            u32x2 pr[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                f32x4 s[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int d = 0; d < DS; ++d) s[u] = M::mma16(kr[u][d], q[n][d], s[u]);
-                }
                 if (!whole) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int key = k0 + 16 * (i >> 2) + 4 * g + (i & 3);
-                        const bool sees = !bad[i >> 2] && key < hi[n] && key >= lo[n] && key < end;
-                        s[i >> 2][i & 3] = sees ? s[i >> 2][i & 3] : kNone;
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = k0 + 4 * g + i;
+                        const bool sees = !bad & (key < hi[n]) & (key >= lo[n]) & (key < w_end);
+                        s[n][i] = sees ? s[n][i] : kNone;
                     }
                 }
-                float t = s[0][0];
-#pragma unroll
-                for (int i = 1; i < 8; ++i) t = fmaxf(t, s[i >> 2][i & 3]);
-                t *= c;
+                float t = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])) * c;
                 if (__ballot(t > m[n] + kSlack) != 0) {
                     t = fmaxf(t, __shfl_xor(t, 16));
                     t = fmaxf(t, __shfl_xor(t, 32));
@@ -228,25 +267,48 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
                     for (int j = 0; j < DJ; ++j) o[n][j] *= f;
                 }
                 const float sub = m[n] == kNone ? 0.0f : m[n];
-                float e[8];
+                float e[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], c, -sub));
-                    l[n] += e[i];
-                }
-                // rounded to the values' type for the product, as the sum is not: within half a step of each term
-                pr[n] = u32x4{M::pack2(e[0], e[1]), M::pack2(e[2], e[3]), M::pack2(e[4], e[5]), M::pack2(e[6], e[7])};
+                for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c, -sub));
+                // rounded to the values' type for the product; the sum takes the rounded ones too (as in the tile kernel)
+                pr[n] = u32x2{M::pack2(e[0], e[1]), M::pack2(e[2], e[3])};
+                l[n] = M::add2(pr[n][1], M::add2(pr[n][0], l[n]));
             }
+            if (sent) wait_vmcnt<3 * kCopies>();
+            else if (left > kFewKeys) wait_vmcnt<2 * kCopies>();
+            else wait_vmcnt<0>();
 #pragma unroll
             for (int j = 0; j < DJ; ++j) {
-                // V^T's rows d = (D / 16) col + j, or 8 col + j % 8 of each 128 where a lane has several vectors
-                const int w = j / 2;
-                const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
-                u32x4 a;
+                const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_turned)(vaddr[j] + kBase));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(vr[2 * i + 1][w], vr[2 * i][w], sel);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) o[n][j] = M::mma16(a, pr[n], o[n][j]);
+                for (int n = 0; n < NT; ++n) o[n][j] = M::mma16_short(a, pr[n], o[n][j]);
+            }
+            if (sent) copy_values(next, decltype(which)::value);
+        };
+        wait_all_loads();  // the queries: the waits below count copies only
+        __syncthreads();   // the rings held the waves' results of the rows before
+        if (w_begin < w_end) {
+            Run r{w_begin, w_begin / page_size, 0, -1};
+            r.slot = w_begin - r.blk * page_size;
+            look(r);
+            copy_keys(r, 0);
+            copy_values(r, 0);
+            bool bad0 = r.page < 0, bad1 = true;
+            walk(r);
+            if (r.key < w_end) {
+                copy_keys(r, 1);
+                copy_values(r, 1);
+                bad1 = r.page < 0;
+                walk(r);
+            }
+            for (int k0 = w_begin; k0 < w_end; k0 += 2 * kFewKeys) {
+                step(k0, w_end - k0, bad0, r, std::integral_constant<int, 0>{});
+                bad0 = r.page < 0;
+                walk(r);
+                if (k0 + kFewKeys >= w_end) break;
+                step(k0 + kFewKeys, w_end - k0 - kFewKeys, bad1, r, std::integral_constant<int, 1>{});
+                bad1 = r.page < 0;
+                walk(r);
             }
         }
         // the waves' results, one set of 16 rows after the other
@@ -260,9 +322,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
             for (int j = 0; j < DJ; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int row = 4 * g + r;  // of V^T's 16: the column that this row's lane loaded
-                    const int d = VC == 0 ? (D / 16) * row + j : 128 * (j / 8) + 8 * row + j % 8;
-                    lds_o[wave][col * D + (d ^ (col & 7) * 4)] = o[n][j][r];
+                    const int d = 16 * j + 4 * g + r;
+                    lds_o[wave * 16 * D + col * D + (d ^ (col & 7) * 4)] = o[n][j][r];
                 }
             __syncthreads();
             constexpr int kPer = 64 * kFewWaves / 16;  // threads that share a row
@@ -283,7 +344,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
                     f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int w = 0; w < kFewWaves; ++w)
-                        v += f[w] * *reinterpret_cast<const f32x4*>(&lds_o[w][my * D + (d ^ (my & 7) * 4)]);
+                        v += f[w] * *reinterpret_cast<const f32x4*>(&lds_o[w * 16 * D + my * D + (d ^ (my & 7) * 4)]);
                     if (plan.splits > 1)
                         *reinterpret_cast<f32x4*>(plan.part + (at * plan.splits + blockIdx.x) * D + d) = v;
                     else
@@ -308,8 +369,6 @@ struct TileSize {
     static constexpr int kKeys = D <= 128 ? 64 : 32;
     static constexpr int kBytes = kKeys * D * 2;
 };
-
-__device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
 
 // Which tile of which sequence workgroup `i` has: tiles are numbered over the sequences with more than few_rows rows.
 struct TileId {
@@ -698,8 +757,9 @@ static hipError_t attention_d(const AttentionParams& p, hipStream_t s) {
     }
     if (f.few) {
         const dim3 grid(f.splits, p.kv_heads, p.step.seqs);
-        if (f.most <= 16) hipLaunchKernelGGL((attend_few_kernel<M, D, 1>), grid, dim3(64 * kFewWaves), 0, s, p, plan);
-        else hipLaunchKernelGGL((attend_few_kernel<M, D, 2>), grid, dim3(64 * kFewWaves), 0, s, p, plan);
+        const int lds = kFewWaves * 4 * kFewKeys * D * 2;  // the rings; the results of 16 rows take half of it
+        if (f.most <= 16) hipLaunchKernelGGL((attend_few_kernel<M, D, 1>), grid, dim3(64 * kFewWaves), lds, s, p, plan);
+        else hipLaunchKernelGGL((attend_few_kernel<M, D, 2>), grid, dim3(64 * kFewWaves), lds, s, p, plan);
     }
     if (f.splits > 1) {
         const long long rows = (long long)p.step.tokens * p.q.heads;
