@@ -98,6 +98,19 @@ __device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
 constexpr int kFewWaves = 4;
 constexpr int kFewKeys = 16;
 constexpr int kFewLeast = 256;  // keys of a split
+constexpr int kFewSlots = 512;
+
+// Keys of a split of the few-rows kernel: what gives the card's workgroups equal shares of all sequences' keys, whose number only the
+// device knows. Asked by whole waves.
+__device__ __forceinline__ int few_least(const AttentionParams& p) {
+    long long keys = 0;
+    for (int b = threadIdx.x & 63; b < p.step.seqs; b += 64) {
+        const int n = min(max(p.step.lengths[b], 0), p.step.blocks * p.step.page_size);
+        keys += p.window > 0 ? min(n, p.window) : n;
+    }
+    const float sum = wave_sum((float)keys) * (float)p.kv_heads;
+    return __builtin_amdgcn_readfirstlane(max(kFewLeast, (int)fminf(sum / kFewSlots, 1.0e9f)));
+}
 
 template <class M, int D, int NT>
 __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionParams p, AttentionPlan plan) {
@@ -114,7 +127,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
     __shared__ float2 lds_ml[kFewWaves][16];
     float* lds_o = reinterpret_cast<float*>(lds);  // [wave][16 * D]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const int b = blockIdx.z, kh = blockIdx.y;
+    const int b = blockIdx.y, kh = blockIdx.x, split = blockIdx.z;
     const int group = p.q.heads / p.kv_heads;
     int first, count;
     step_tokens(p.step, b, first, count);
@@ -125,6 +138,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
     const char* vbase = static_cast<const char*>(p.v.p) + 2 * kh * p.v.head;
     const auto* table = (const __attribute__((address_space(4))) int32_t*)(p.step.table + b * p.step.table_stride);
     const float c = p.scale * kLog2e;
+    const int least = plan.splits > 1 ? few_least(p) : 0;
     // from a copy's first row: this lane's row, and the vector that belongs at its place
     const int crow = lane / CH, cpos = lane % CH;
     uint32_t koff[kCopies], voff[kCopies];
@@ -178,7 +192,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
         all_hi = __builtin_amdgcn_readfirstlane(all_hi);
         all_lo = __builtin_amdgcn_readfirstlane(all_lo);
         int begin, end;
-        split_range(least_lo & ~(kFewKeys - 1), most_hi, blockIdx.x, plan.splits, kFewKeys * kFewWaves, kFewLeast, begin, end);
+        split_range(least_lo & ~(kFewKeys - 1), most_hi, split, plan.splits, kFewKeys * kFewWaves, least, begin, end);
         // this wave's quarter of them; a stage lies inside one page (pages hold a multiple of 16 slots), and the pages are walked along
         // the table without a division
         const int quarter = (end - begin + kFewKeys * kFewWaves - 1) / (kFewKeys * kFewWaves) * kFewKeys;
@@ -285,8 +299,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
             }
             if (sent) copy_values(next, decltype(which)::value);
         };
-        wait_all_loads();  // the queries: the waits below count copies only
-        __syncthreads();   // the rings held the waves' results of the rows before
+        __syncthreads();  // the rings held the waves' results of the rows before
         if (w_begin < w_end) {
             Run r{w_begin, w_begin / page_size, 0, -1};
             r.slot = w_begin - r.blk * page_size;
@@ -301,6 +314,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
                 bad1 = r.page < 0;
                 walk(r);
             }
+            wait_all_loads();  // the queries too: the waits in the loop count copies only
             for (int k0 = w_begin; k0 < w_end; k0 += 2 * kFewKeys) {
                 step(k0, w_end - k0, bad0, r, std::integral_constant<int, 0>{});
                 bad0 = r.page < 0;
@@ -346,12 +360,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
                     for (int w = 0; w < kFewWaves; ++w)
                         v += f[w] * *reinterpret_cast<const f32x4*>(&lds_o[w * 16 * D + my * D + (d ^ (my & 7) * 4)]);
                     if (plan.splits > 1)
-                        *reinterpret_cast<f32x4*>(plan.part + (at * plan.splits + blockIdx.x) * D + d) = v;
+                        *reinterpret_cast<f32x4*>(plan.part + (at * plan.splits + split) * D + d) = v;
                     else
                         *reinterpret_cast<u32x2*>(static_cast<raw*>(p.out) + at * D + d) =
                             u32x2{M::pack2(v[0] * k, v[1] * k), M::pack2(v[2] * k, v[3] * k)};
                 }
-                if (plan.splits > 1 && part == 0) plan_stats(plan, p)[at * plan.splits + blockIdx.x] = make_float2(mx, sum);
+                if (plan.splits > 1 && part == 0) plan_stats(plan, p)[at * plan.splits + split] = make_float2(mx, sum);
             }
         }
     }
@@ -630,12 +644,11 @@ __global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile
         if (more) weigh(which, std::true_type{});
         else weigh(which, std::false_type{});
     };
-    wait_all_loads();  // the queries: a wait for them inside the loop would be one for the copies too
     if (begin < end) {
         copy_keys(0);
         copy_values(0, vr);
         vr = kr;
-        wait_vmcnt<0>();
+        wait_all_loads();  // the queries too: a wait for them inside the loop would be one for the copies sent there
         __syncthreads();
         if (begin + KT < end) copy_keys(1);
         if (!idle) scores(std::integral_constant<int, 0>{});
@@ -756,7 +769,8 @@ static hipError_t attention_d(const AttentionParams& p, hipStream_t s) {
         hipLaunchKernelGGL((attend_tile_kernel<M, D>), dim3(f.tiles * p.kv_heads, f.splits), dim3(64 * kTileWaves), lds, s, p, plan);
     }
     if (f.few) {
-        const dim3 grid(f.splits, p.kv_heads, p.step.seqs);
+        // splits slowest: the workgroups of one split number spread over the XCDs, and those without keys come last
+        const dim3 grid(p.kv_heads, p.step.seqs, f.splits);
         const int lds = kFewWaves * 4 * kFewKeys * D * 2;  // the rings; the results of 16 rows take half of it
         if (f.most <= 16) hipLaunchKernelGGL((attend_few_kernel<M, D, 1>), grid, dim3(64 * kFewWaves), lds, s, p, plan);
         else hipLaunchKernelGGL((attend_few_kernel<M, D, 2>), grid, dim3(64 * kFewWaves), lds, s, p, plan);
