@@ -202,8 +202,8 @@ __global__ __launch_bounds__(kWideThreads) void norm_wide_kernel(NormParams p) {
 // read once more), else one per `groups` rows.
 constexpr int kBackBlocks = 512;
 
-template <class T, class W, int NC>
-__global__ __launch_bounds__(64 * kWaves) void norm_back_kernel(NormParams p, int gw) {
+template <class T, class W, int NC, bool BIAS>
+__global__ __launch_bounds__(64 * kWaves, 4) void norm_back_kernel(NormParams p, int gw) {
     constexpr int V = T::kVec;
     extern __shared__ float sums[];  // [NC * gw * 64 * V], at most 48 KB
     __shared__ float lds[2][2 * kWaves];
@@ -211,11 +211,11 @@ __global__ __launch_bounds__(64 * kWaves) void norm_back_kernel(NormParams p, in
     const int first = (wave & (gw - 1)) * 64 + (threadIdx.x & 63), step = 64 * gw;
     const int cols = p.cols;
     const float inv = 1.0f / (float)cols;
-    float dw[NC][V], db[NC][V];
+    float dw[NC][V], db[BIAS ? NC : 1][V];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int i = 0; i < V; ++i) dw[c][i] = db[c][i] = 0.0f;
+        for (int i = 0; i < V; ++i) dw[c][i] = db[BIAS ? c : 0][i] = 0.0f;
     int turn = 0;
     for (long long r0 = (long long)blockIdx.x * groups; r0 < p.rows; r0 += (long long)gridDim.x * groups, turn ^= 1) {
         const long long row = r0 + group;
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(64 * kWaves) void norm_back_kernel(NormParams p, in
                     const float h = (f[i] - mean) * rstd;
                     const float gw_ = g[i] * w[i];  // 0 past the row's end, where dy and w are read as 0
                     dw[c][i] += g[i] * h;
-                    db[c][i] += g[i];
+                    if constexpr (BIAS) db[c][i] += g[i];
                     s[0] += gw_;
                     s[1] += gw_ * h;
                 }
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(64 * kWaves) void norm_back_kernel(NormParams p, in
     const int width = NC * step;
     float* part = p.partial + (long long)blockIdx.x * 2 * cols;
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
+    for (int which = 0; which < (BIAS ? 2 : 1); ++which) {
         for (int t = 0; t < groups; ++t) {
             __syncthreads();
             if (group == t) {
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(64 * kWaves) void norm_back_kernel(NormParams p, in
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         const int at = i * width + c * step + first;  // consecutive lanes on consecutive banks
-                        const float v = which ? db[c][i] : dw[c][i];
+                        const float v = which ? db[BIAS ? c : 0][i] : dw[c][i];
                         sums[at] = t ? sums[at] + v : v;
                     }
             }
@@ -350,22 +350,25 @@ __global__ __launch_bounds__(256) void norm_strip_kernel(NormParams p) {
     part[p.cols + j] = db;
 }
 
-// dweight and dbias from the partial rows, in their order: 16 threads a column take every 16th row each, then one adds the 16.
+// dweight and dbias from the partial rows, in their order: 32 threads a column take every 32nd row each, then one adds the 32.
 template <class W>
 __global__ __launch_bounds__(1024) void norm_fold_kernel(NormParams p, int rows) {
-    __shared__ float lds[16][65];
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+    __shared__ float lds[32][33];
+    const int c = threadIdx.x & 31, part = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
     const int which = blockIdx.y;  // 0: dweight, 1: dbias
-    float v = 0.0f;
-    if (col < p.cols)
-        for (int r = part; r < rows; r += 16) v += p.partial[((long long)r * 2 + which) * p.cols + col];
-    lds[part][threadIdx.x & 63] = v;
-    __syncthreads();
     void* out = which ? p.dbias : p.dweight;
+    float v = 0.0f;
+    if (col < p.cols && out) {
+        const float* src = p.partial + (long long)which * p.cols + col;
+#pragma unroll 16
+        for (int r = part; r < rows; r += 32) v += src[(long long)r * 2 * p.cols];
+    }
+    lds[part][c] = v;
+    __syncthreads();
     if (part || col >= p.cols || !out) return;
     v = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) v += lds[r][threadIdx.x & 63];
+    for (int r = 0; r < 32; ++r) v += lds[r][c];
     static_cast<typename W::raw*>(out)[col] = W::put(v);
 }
 
@@ -419,16 +422,22 @@ static void norm_backward(const NormParams& p, hipStream_t s) {
         NormParams q = p;
         if (!sums) q.partial = nullptr;
         const int nc = ceil_div(ceil_div(p.cols, T::kVec), 64 * gw);
-#define CMOE_BACK(NC)                                                                                                  \
-    hipLaunchKernelGGL((norm_back_kernel<T, W, NC>), dim3(parts), dim3(64 * kWaves), sums ? 4 * NC * gw * 64 * T::kVec : 0, s, q, gw)
-        if (nc <= 1) CMOE_BACK(1);
-        else if (nc == 2) CMOE_BACK(2);
-        else CMOE_BACK(3);
+#define CMOE_BACK(NC, BIAS) \
+    hipLaunchKernelGGL((norm_back_kernel<T, W, NC, BIAS>), dim3(parts), dim3(64 * kWaves), sums ? 4 * NC * gw * 64 * T::kVec : 0, s, q, gw)
+        if (p.dbias) {
+            if (nc <= 1) CMOE_BACK(1, true);
+            else if (nc == 2) CMOE_BACK(2, true);
+            else CMOE_BACK(3, true);
+        } else {
+            if (nc <= 1) CMOE_BACK(1, false);
+            else if (nc == 2) CMOE_BACK(2, false);
+            else CMOE_BACK(3, false);
+        }
 #undef CMOE_BACK
     } else if (sums) {
         hipLaunchKernelGGL((norm_strip_kernel<T>), dim3(ceil_div(p.cols, 256), parts), dim3(256), 0, s, p);
     }
-    if (sums) hipLaunchKernelGGL((norm_fold_kernel<W>), dim3(ceil_div(p.cols, 64), p.dbias ? 2 : 1), dim3(1024), 0, s, p, parts);
+    if (sums) hipLaunchKernelGGL((norm_fold_kernel<W>), dim3(ceil_div(p.cols, 32), p.dbias ? 2 : 1), dim3(1024), 0, s, p, parts);
 }
 
 hipError_t launch_norm(const NormParams& p, hipStream_t s) {
