@@ -30,6 +30,7 @@ _CACHE_DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYP
 _FREQ_DTYPES = {torch.float32: _native.DTYPE_F32, torch.float64: _native.DTYPE_F64}
 _POSITION_DTYPES = {torch.int32: _native.INDEX_I32, torch.int64: _native.INDEX_I64}
 _Strides = ctypes.c_int64 * 6
+_ATTENTION_DIMS = (64, 128, 256)
 
 
 def _ptr(t):
@@ -38,6 +39,11 @@ def _ptr(t):
 
 def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _refuse_gradient(what, *tensors) -> None:
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
 
 
 # ---- layer norm ---------------------------------------------------------------------------------------------------------
@@ -55,6 +61,18 @@ def _check_norm(x, weight, bias):
              "weight and bias must be [N] for x [..., N]")
     _require(x.is_contiguous() and weight.is_contiguous() and (bias is None or bias.is_contiguous()),
              "x, weight and bias must be contiguous")
+
+
+def _norm_ok(x, weight, bias) -> bool:
+    """Whether a call holds to _check_norm's contract, in one expression on every short call's path; what it refuses goes to
+    _check_norm, which says what is wrong. A condition added there belongs here too."""
+    try:
+        dev, dt, wt, n = x.get_device(), x.dtype, weight.dtype, weight.shape
+        return (dev >= 0 and dt in _DTYPES and (wt is dt or wt is torch.float32) and len(n) == 1 and n[0] > 0 and x.shape[-1:] == n
+                and weight.get_device() == dev and x.is_contiguous() and weight.is_contiguous()
+                and (bias is None or (bias.dtype is wt and bias.shape == n and bias.get_device() == dev and bias.is_contiguous())))
+    except (AttributeError, TypeError):
+        return False
 
 
 def _norm_forward(x, weight, bias, eps, keep_stats):
@@ -99,7 +117,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     """(x - mean) / sqrt(var + eps) * weight (+ bias) over x's last dimension, x [..., N] bf16, fp16 or fp32; weight and bias [N] in
     x's type or fp32. Sums are fp32 and the result is rounded once. Differentiable in x, weight and bias; the gradients are the
     same bits every run."""
-    _check_norm(x, weight, bias)
+    if not _norm_ok(x, weight, bias):
+        _check_norm(x, weight, bias)
     if _wants_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _norm_forward(x, weight, bias, float(eps), False)[0]
@@ -168,6 +187,36 @@ def _check_frequencies(inv_freq, dim, device):
     _require(2 * inv_freq.numel() <= dim, "inv_freq must hold at most dim / 2 frequencies")
 
 
+def _check_rotary(q, k, positions, inv_freq):
+    _require(isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _DTYPES, "q must be a bfloat16, float16 or float32 CUDA (HIP) tensor")
+    _check_heads(q, "q", None, None, q)
+    if k is not None:
+        _check_heads(k, "k", q.size(0), q.size(2), q)
+    _check_frequencies(inv_freq, q.size(2), q.device)
+    _require(isinstance(positions, torch.Tensor) and positions.device == q.device and positions.dtype in _POSITION_DTYPES
+             and positions.shape == q.shape[:1] and positions.is_contiguous(),
+             "positions must be a contiguous int32 or int64 [tokens] tensor on the same device")
+
+
+def _frequencies_ok(inv_freq, dim, dev) -> bool:
+    return (inv_freq.get_device() == dev and inv_freq.dtype in _FREQ_DTYPES and inv_freq.dim() == 1 and inv_freq.is_contiguous()
+            and 2 * inv_freq.numel() <= dim)
+
+
+def _rotary_ok(q, k, positions, inv_freq) -> bool:
+    """_check_rotary's contract in one expression (as _norm_ok)."""
+    try:
+        tokens, _, dim = q.shape
+        dev, dt = q.get_device(), q.dtype
+        return (dev >= 0 and dt in _DTYPES and q.stride(2) == 1
+                and (k is None or (k.dim() == 3 and k.size(0) == tokens and k.size(2) == dim and k.stride(2) == 1 and k.dtype is dt
+                                   and k.get_device() == dev))
+                and _frequencies_ok(inv_freq, dim, dev) and positions.get_device() == dev and positions.dtype in _POSITION_DTYPES
+                and positions.shape == (tokens,) and positions.is_contiguous())
+    except (AttributeError, TypeError, ValueError):
+        return False
+
+
 def _rotary_launch(q, k, positions, inv_freq, interleaved, scale, backward):
     first = q if q is not None else k
     tokens, _, dim = first.shape
@@ -205,14 +254,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     strides. The first 2 * len(inv_freq) elements of a head are pairs, elements (2i, 2i + 1) if ``interleaved``, (i, i + pairs) if
     not; pair i turns by positions[t] * inv_freq[i] and is multiplied by ``scale``; the rest of the head is copied. Angles are
     formed in 64 bits, so positions of a million lose nothing. Differentiable in q and k."""
-    _require(isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _DTYPES, "q must be a bfloat16, float16 or float32 CUDA (HIP) tensor")
-    _check_heads(q, "q", None, None, q)
-    if k is not None:
-        _check_heads(k, "k", q.size(0), q.size(2), q)
-    _check_frequencies(inv_freq, q.size(2), q.device)
-    _require(isinstance(positions, torch.Tensor) and positions.device == q.device and positions.dtype in _POSITION_DTYPES
-             and positions.shape == q.shape[:1] and positions.is_contiguous(),
-             "positions must be a contiguous int32 or int64 [tokens] tensor on the same device")
+    if not _rotary_ok(q, k, positions, inv_freq):
+        _check_rotary(q, k, positions, inv_freq)
     if _wants_grad(q, k):
         return _Rotary.apply(q, k, positions, inv_freq, int(bool(interleaved)), float(scale))
     return tuple(_rotary_launch(q, k, positions, inv_freq, int(bool(interleaved)), float(scale), 0))
@@ -245,6 +288,79 @@ def _check_step(like, k_pages, v_pages, block_table, lengths, q_offsets, tokens,
                  "q_offsets must be contiguous int32 [sequences + 1] on the step's device")
 
 
+def _step_ok(like, k_pages, v_pages, block_table, lengths, q_offsets, tokens, dim, kv_heads) -> bool:
+    """_check_step's contract in one expression (as _norm_ok); the caller catches what a wrong type raises."""
+    dev, dt = like.get_device(), like.dtype
+    pages, page_size, heads, d = shape = k_pages.shape
+    seqs, blocks = block_table.shape
+    return (dev >= 0 and dt in _CACHE_DTYPES and d == dim and (kv_heads is None or heads == kv_heads) and v_pages.shape == shape
+            and k_pages.dtype is dt and v_pages.dtype is dt and k_pages.get_device() == dev and v_pages.get_device() == dev
+            and k_pages.stride(3) == 1 and v_pages.stride(3) == 1 and pages >= 1 and page_size >= 16 and page_size % 16 == 0
+            and block_table.dtype is torch.int32 and block_table.get_device() == dev and (block_table.stride(1) == 1 or blocks <= 1)
+            and lengths.dtype is torch.int32 and lengths.get_device() == dev and lengths.shape == (seqs,) and lengths.is_contiguous()
+            and (tokens % max(seqs, 1) == 0 if q_offsets is None else
+                 (q_offsets.dtype is torch.int32 and q_offsets.get_device() == dev and q_offsets.shape == (seqs + 1,)
+                  and q_offsets.is_contiguous())))
+
+
+def _heads_ok(t, tokens, dim, like) -> bool:
+    return (t.dim() == 3 and t.size(0) == tokens and t.size(2) == dim and t.stride(2) == 1 and t.dtype is like.dtype
+            and t.get_device() == like.get_device())
+
+
+def _append_ok(k, v, k_pages, v_pages, block_table, lengths, q_offsets, q, inv_freq) -> bool:
+    try:
+        tokens, kv_heads, dim = k.shape
+        return (k.stride(2) == 1 and _heads_ok(v, tokens, dim, k) and v.size(1) == kv_heads
+                and (q is None or _heads_ok(q, tokens, dim, k))
+                and _step_ok(k, k_pages, v_pages, block_table, lengths, q_offsets, tokens, dim, kv_heads)
+                and (inv_freq is None or _frequencies_ok(inv_freq, dim, k.get_device())))
+    except (AttributeError, TypeError, ValueError):
+        return False
+
+
+def _check_append(k, v, k_pages, v_pages, block_table, lengths, q_offsets, q, inv_freq):
+    _require(all(isinstance(t, torch.Tensor) for t in (k, v)) and (q is None or isinstance(q, torch.Tensor)),
+             "q, k and v must be tensors")
+    _check_heads(k, "k", None, None, k)
+    tokens, kv_heads, dim = k.shape
+    _check_heads(v, "v", tokens, dim, k)
+    _require(v.size(1) == kv_heads, "k and v must have the same heads")
+    if q is not None:
+        _check_heads(q, "q", tokens, dim, k)
+    _check_step(k, k_pages, v_pages, block_table, lengths, q_offsets, tokens, dim, kv_heads)
+    if inv_freq is not None:
+        _check_frequencies(inv_freq, dim, k.device)
+
+
+def _attention_ok(q, k_pages, v_pages, block_table, lengths, q_offsets, sinks, out) -> bool:
+    try:
+        tokens, heads, dim = q.shape
+        kv_heads = k_pages.size(2)
+        return (q.stride(2) == 1 and dim in _ATTENTION_DIMS and kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0
+                and _step_ok(q, k_pages, v_pages, block_table, lengths, q_offsets, tokens, dim, None)
+                and (sinks is None or (sinks.dtype is torch.float32 and sinks.shape == (heads,) and sinks.is_contiguous()
+                                       and sinks.get_device() == q.get_device()))
+                and (out is None or (_heads_ok(out, tokens, dim, q) and out.size(1) == heads and out.is_contiguous())))
+    except (AttributeError, TypeError, ValueError):
+        return False
+
+
+def _check_attention(q, k_pages, v_pages, block_table, lengths, q_offsets, sinks, out):
+    _require(isinstance(q, torch.Tensor), "q must be a tensor")
+    _check_heads(q, "q", None, None, q)
+    tokens, heads, dim = q.shape
+    _check_step(q, k_pages, v_pages, block_table, lengths, q_offsets, tokens, dim, None)
+    kv_heads = k_pages.size(2)
+    _require(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "q's heads must be a multiple of the pages' heads")
+    _require(dim in _ATTENTION_DIMS, "paged_attention takes head sizes 64, 128 and 256")
+    _require(sinks is None or (isinstance(sinks, torch.Tensor) and sinks.device == q.device and sinks.dtype == torch.float32
+                               and sinks.shape == (heads,) and sinks.is_contiguous()),
+             "sinks must be contiguous float32 [heads] on q's device")
+    _require(out is None or (isinstance(out, torch.Tensor) and out.device == q.device and out.dtype == q.dtype and out.is_contiguous()
+                             and out.shape == q.shape), "out must be a contiguous tensor of q's shape, type and device")
+
+
 def _pages_args(k_pages, v_pages):
     return _Strides(*k_pages.stride()[:3], *v_pages.stride()[:3]), k_pages.size(0), k_pages.size(1)
 
@@ -261,19 +377,13 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     """Writes the step's keys and values [tokens, kv_heads, dim] to their slots of the pages, the keys turned to their positions as
     ``rotary`` does where ``inv_freq`` is given. ``q`` [tokens, heads, dim] is turned in the same launch and returned as a new
     tensor (None without q). A position past the table's end is not written."""
-    tensors = [t for t in (k, v, q) if t is not None]
-    _require(all(isinstance(t, torch.Tensor) for t in tensors), "q, k and v must be tensors")
-    _require(not _wants_grad(*tensors, k_pages, v_pages), "paged_append has no backward pass: call it under torch.no_grad()")
-    _check_heads(k, "k", None, None, k)
+    if not _append_ok(k, v, k_pages, v_pages, block_table, lengths, q_offsets, q, inv_freq):
+        _refuse_gradient("paged_append", q, k, v, k_pages, v_pages)
+        _check_append(k, v, k_pages, v_pages, block_table, lengths, q_offsets, q, inv_freq)
+    _refuse_gradient("paged_append", q, k, v, k_pages, v_pages)
     tokens, kv_heads, dim = k.shape
-    _check_heads(v, "v", tokens, dim, k)
-    _require(v.size(1) == kv_heads, "k and v must have the same heads")
-    if q is not None:
-        _check_heads(q, "q", tokens, dim, k)
-    _check_step(k, k_pages, v_pages, block_table, lengths, q_offsets, tokens, dim, kv_heads)
     pairs = freq = 0
     if inv_freq is not None:
-        _check_frequencies(inv_freq, dim, k.device)
         pairs, freq = inv_freq.numel(), _FREQ_DTYPES[inv_freq.dtype]
     out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     seqs = block_table.size(0)
@@ -296,32 +406,25 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     consecutive groups. ``scale`` (default 1 / sqrt(dim)) multiplies the scores. ``sinks`` [heads] fp32 is one more score per head that
     takes weight and has no value. A row that sees nothing is 0. ``max_new`` is the largest number of new tokens of a sequence, where
     the caller knows it: it picks the kernels, and the result holds for any value. Head sizes 64, 128 and 256."""
-    _require(isinstance(q, torch.Tensor), "q must be a tensor")
-    _require(not _wants_grad(q, k_pages, v_pages, sinks), "paged_attention has no backward pass: call it under torch.no_grad()")
-    _check_heads(q, "q", None, None, q)
+    if not _attention_ok(q, k_pages, v_pages, block_table, lengths, q_offsets, sinks, out):
+        _refuse_gradient("paged_attention", q, k_pages, v_pages, sinks)
+        _check_attention(q, k_pages, v_pages, block_table, lengths, q_offsets, sinks, out)
+    _refuse_gradient("paged_attention", q, k_pages, v_pages, sinks)
     tokens, heads, dim = q.shape
-    _check_step(q, k_pages, v_pages, block_table, lengths, q_offsets, tokens, dim, None)
     kv_heads = k_pages.size(2)
-    _require(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "q's heads must be a multiple of the pages' heads")
-    _require(dim in (64, 128, 256), "paged_attention takes head sizes 64, 128 and 256")
     _require(window >= 0, "window must not be negative")
     scale = dim ** -0.5 if scale is None else float(scale)
     _require(0.0 < scale < math.inf, "scale must be positive")
-    if sinks is not None:
-        _require(isinstance(sinks, torch.Tensor) and sinks.device == q.device and sinks.dtype == torch.float32
-                 and sinks.shape == (heads,) and sinks.is_contiguous(), "sinks must be contiguous float32 [heads] on q's device")
     if out is None:
         out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
-    else:
-        _require(isinstance(out, torch.Tensor) and out.device == q.device and out.dtype == q.dtype and out.is_contiguous()
-                 and out.shape == q.shape, "out must be a contiguous tensor of q's shape, type and device")
     seqs, blocks, page_size = block_table.size(0), block_table.size(1), k_pages.size(1)
     if tokens and seqs:
         L = _native.lib()
         most = int(max_new) if max_new is not None else 0
         nbytes = L.cernels_paged_attention_workspace_bytes(tokens, seqs, heads, kv_heads, dim, page_size, blocks, most)
-        _require(nbytes > 0, f"cernels_paged_attention: invalid dimensions tokens={tokens} heads={heads}/{kv_heads} dim={dim} "
-                             f"sequences={seqs} blocks={blocks} x {page_size}")
+        if nbytes == 0:
+            raise RuntimeError(f"cernels_paged_attention: invalid dimensions tokens={tokens} heads={heads}/{kv_heads} dim={dim} "
+                               f"sequences={seqs} blocks={blocks} x {page_size}, max_new={max_new}")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         _launch("cernels_paged_attention", q.get_device(), L.cernels_paged_attention, q.data_ptr(), q.stride(0), q.stride(1), heads,
                 kv_heads, dim, _CACHE_DTYPES[q.dtype], k_pages.data_ptr(), v_pages.data_ptr(), *_pages_args(k_pages, v_pages),
