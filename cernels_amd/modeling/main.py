@@ -12,7 +12,8 @@ swap entry, stock first, is
   - timed for decode (tokens per second of a fixed-length greedy generate, prefill subtracted).
 Two correct bf16 implementations drift apart on a deep model too, so the same two gate numbers are
 also measured between stock and stock under transformers' other experts implementation
-(``stock_drift_calibration``). The model is the real transformers architecture, from a local
+(``stock_drift_calibration``). ``--paged`` adds the last variant run on a paged cache
+(cernels_amd.modeling.paged). The model is the real transformers architecture, from a local
 checkpoint directory or with seeded random weights (cernels_amd.modeling.models), fed seeded random
 token ids. The result is written as JSON to ``<out>/<host>/model/<model>.json`` (``--out``, default
 ``analysis``; ``python -m cernels_amd.modeling.view`` tabulates the saved results) and printed.
@@ -158,6 +159,9 @@ def main(argv=None):
     ap.add_argument("--min-run-time", type=float, default=Options.prefill_seconds,
                     help="seconds of prefill timing per variant")
     ap.add_argument("--variants", help="comma list (stock is always first)")
+    ap.add_argument("--paged", action="store_true",
+                    help="also run the decoder layers on a paged cache (cernels_amd.modeling.paged) with the last variant's experts, "
+                         "as variant <name>_paged")
     ap.add_argument("--stock-experts", choices=["default", "eager", "grouped_mm"], default="default",
                     help="transformers experts implementation of the stock variant")
     ap.add_argument("--out", default="analysis", help="root of the saved results: <out>/<host>/model/<model>.json")
@@ -181,6 +185,17 @@ def main(argv=None):
     variants = None if not args.variants else [v.strip() for v in args.variants.split(",") if v.strip()]
     opts = Options(args.gate_tokens, args.decode_tokens, args.runs, args.min_run_time)
     results = sweep(model, inputs, args.model, variants, opts)
+    if args.paged:
+        from cernels_amd.modeling import paged
+
+        last = list(results)[-1]
+        reference = trace(model, inputs, opts.gate_tokens)
+        SWAPS[args.model][0](model, last)
+        try:
+            results[f"{last}_paged"] = paged.measure(model, inputs, opts, reference)
+        finally:
+            SWAPS[args.model][0](model, "stock")
+        _log(f"{last}_paged: {results[f'{last}_paged']}")
     drift = stock_drift(model, inputs, args.gate_tokens)
     _log(f"stock drift calibration ({cfg._experts_implementation} vs {drift['other']}): {drift}")
     payload = {
