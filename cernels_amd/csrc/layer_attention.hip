@@ -25,6 +25,7 @@ constexpr float kNone = -__builtin_inff();
 
 struct MathBf16 {
     typedef TypeBf16 T;
+    static constexpr uint32_t kExponent = 0x7f80;
     static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
@@ -42,6 +43,7 @@ struct MathBf16 {
 };
 struct MathF16 {
     typedef TypeF16 T;
+    static constexpr uint32_t kExponent = 0x7c00;
     static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
@@ -58,6 +60,35 @@ struct MathF16 {
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), __builtin_bit_cast(f16x2, 0x3c003c00u), sum, false);
     }
 };
+
+// Values that are not finite, in tiles of which some rows do not see some keys: a key that a row does not see has probability 0 there,
+// but 0 times an infinity is a NaN. Such tiles (the last ones of a row's keys and the first ones of its window) are looked through, and
+// from one that holds such a value on, a wave goes through its keys one by one, adding to each row what it sees and nothing else.
+template <class M>
+__device__ __forceinline__ uint32_t not_finite(u32x4 v) {  // one of the two top bits is set if a value's exponent is all ones
+    constexpr uint32_t kStep = (0x8000u - M::kExponent) * 0x10001u, kMask = M::kExponent * 0x10001u;
+    uint32_t odd = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) odd |= (v[i] & kMask) + kStep;  // carries into a half's own top bit, no further
+    return odd & 0x80008000u;
+}
+// Part of q k: 8 elements.
+template <class T>
+__device__ __forceinline__ float dot8(const u32x4& a, const u32x4& b, float sum) {
+    float x[8], y[8];
+    T::unpack(a, x);
+    T::unpack(b, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i], y[i], sum);
+    return sum;
+}
+// Raises the maximum to x; what the sums so far, and x, then weigh.
+__device__ __forceinline__ void raise_to(float x, float& m, float& f, float& e) {
+    const float m1 = fmaxf(m, x);
+    f = m1 == kNone ? 1.0f : __builtin_amdgcn_exp2f(m - m1);
+    e = __builtin_amdgcn_exp2f(x - (m1 == kNone ? 0.0f : m1));
+    m = m1;
+}
 
 // What a launch works on beside the call's own parameters.
 struct AttentionPlan {
@@ -255,6 +286,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
 #pragma unroll
                 for (int n = 0; n < NT; ++n) s[n] = M::mma16(a, q[n][d], s[n]);
             }
+            if ((k0 < all_lo || k0 + kFewKeys > all_hi)) {  // some row does not see some key
+                wait_vmcnt<0>();
+                uint32_t odd = 0;
+#pragma unroll
+                for (int at = 0; at < kBytes; at += 1024) odd |= not_finite<M>(*(lds_vec)(ring + kBase + kBytes + at + 16 * lane));
+                if (__ballot(odd != 0) != 0) return true;
+            }
             const bool sent = left > 2 * kFewKeys;
             if (sent) copy_keys(next, decltype(which)::value);
             const bool whole = !bad && k0 >= all_lo && k0 + kFewKeys <= all_hi && left >= kFewKeys;
@@ -298,7 +336,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
                 for (int n = 0; n < NT; ++n) o[n][j] = M::mma16_short(a, pr[n], o[n][j]);
             }
             if (sent) copy_values(next, decltype(which)::value);
+            return false;
         };
+        int resume = w_end;  // the keys from here on are gone through one by one
         __syncthreads();  // the rings held the waves' results of the rows before
         if (w_begin < w_end) {
             Run r{w_begin, w_begin / page_size, 0, -1};
@@ -316,13 +356,46 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
             }
             wait_all_loads();  // the queries too: the waits in the loop count copies only
             for (int k0 = w_begin; k0 < w_end; k0 += 2 * kFewKeys) {
-                step(k0, w_end - k0, bad0, r, std::integral_constant<int, 0>{});
+                if (step(k0, w_end - k0, bad0, r, std::integral_constant<int, 0>{})) {
+                    resume = k0;
+                    break;
+                }
                 bad0 = r.page < 0;
                 walk(r);
                 if (k0 + kFewKeys >= w_end) break;
-                step(k0 + kFewKeys, w_end - k0 - kFewKeys, bad1, r, std::integral_constant<int, 1>{});
+                if (step(k0 + kFewKeys, w_end - k0 - kFewKeys, bad1, r, std::integral_constant<int, 1>{})) {
+                    resume = k0 + kFewKeys;
+                    break;
+                }
                 bad1 = r.page < 0;
                 walk(r);
+            }
+        }
+#pragma unroll 1
+        for (int key = resume; key < w_end; ++key) {
+            Run at{key, key / page_size, 0, -1};
+            at.slot = key - at.blk * page_size;
+            look(at);
+            if (at.page < 0) continue;
+            const char* kp = kbase + 2 * ((long long)at.page * p.k.page + at.slot * p.k.slot);
+            const char* vp = vbase + 2 * ((long long)at.page * p.v.page + at.slot * p.v.slot);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float x = 0.0f;
+#pragma unroll
+                for (int d = 0; d < DS; ++d) x = dot8<T>(*reinterpret_cast<const u32x4*>(kp + 64 * d + 16 * g), q[n][d], x);
+                x += __shfl_xor(x, 16);
+                x = (x + __shfl_xor(x, 32)) * c;
+                if (key < hi[n] && key >= lo[n]) {
+                    float f, e;
+                    raise_to(x, m[n], f, e);
+                    l[n] = l[n] * f + (g == 0 ? e : 0.0f);
+#pragma unroll
+                    for (int j = 0; j < DJ; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            o[n][j][i] = o[n][j][i] * f + e * T::get(reinterpret_cast<const raw*>(vp)[16 * j + 4 * g + i]);
+                }
             }
         }
         // the waves' results, one set of 16 rows after the other
@@ -454,7 +527,7 @@ __global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile
     const int hi = live ? before + token + 1 : 0, lo = low(token);
     const int last_row = min(t.row0 + kTileRows, t.rows) - 1;
     const int w_first = min(t.row0 + 32 * wave, last_row) / group, w_last = min(t.row0 + 32 * wave + 31, last_row) / group;
-    const bool idle = t.row0 + 32 * wave >= t.rows;
+    bool idle = t.row0 + 32 * wave >= t.rows;
     const int w_hi = before + w_last + 1, w_all_hi = before + w_first + 1, w_lo = low(w_first), w_all_lo = low(w_last);
     const int tile_lo = low(t.row0 / group);
     int begin, end;
@@ -627,6 +700,13 @@ __global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile
             }
         }
     };
+    auto odd_values = [&](auto which) __attribute__((always_inline)) {
+        uint32_t odd = 0;
+#pragma unroll 4
+        for (int at = 16 * lane; at < kBytes; at += 1024) odd |= not_finite<M>(*(lds_vec)(lds_u32(lds) + decltype(which)::value * 2 * kBytes + kBytes + at));
+        return __ballot(odd != 0) != 0;
+    };
+    int resume = end;  // the keys from here on are gone through one by one
     // One tile. What was sent a tile ago has landed (its values, the next one's keys); the keys of the tile after that and the next
     // values are sent into the buffers that no wave reads any more.
     auto step = [&](int k0, int tile, auto which) __attribute__((always_inline)) {
@@ -640,6 +720,11 @@ __global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile
             vr = next;
         }
         if (idle) return;
+        if ((k0 < w_all_lo || k0 + KT > w_all_hi) && odd_values(which)) {
+            resume = k0;
+            idle = true;  // of the tiles; the wave still sends its copies
+            return;
+        }
         raise(k0, tile);
         if (more) weigh(which, std::true_type{});
         else weigh(which, std::false_type{});
@@ -658,11 +743,36 @@ __global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile
         if (k0 + KT >= end) break;
         step(k0 + KT, tile + 1, std::integral_constant<int, 1>{});
     }
-    {
-        uint32_t a = __float_as_uint(l), b = a;
+    auto halves = [](float v) __attribute__((always_inline)) {
+        uint32_t a = __float_as_uint(v), b = a;
         swap_halves(a, b);
-        l = __uint_as_float(a) + __uint_as_float(b);
+        return __uint_as_float(a) + __uint_as_float(b);
+    };
+#pragma unroll 1
+    for (int key = resume; key < end; ++key) {
+        const int at = key / page_size, page = page_of(key, at), in = key - at * page_size;
+        if (page < 0) continue;
+        const char* kp = kbase + 2 * ((long long)page * p.k.page + in * p.k.slot);
+        const char* vp = vbase + 2 * ((long long)page * p.v.page + in * p.v.slot);
+        float x = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DS; ++d) x = dot8<T>(*reinterpret_cast<const u32x4*>(kp + 32 * d + 16 * h), q[d], x);
+        x = halves(x) * c;
+        if (key < hi && key >= lo) {
+            float f, e;
+            raise_to(x, m, f, e);
+            l = l * f + (h == 0 ? e : 0.0f);
+#pragma unroll
+            for (int j = 0; j < DT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const raw* v = reinterpret_cast<const raw*>(vp) + 32 * j + 8 * i + 4 * h;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[j][4 * i + r] = o[j][4 * i + r] * f + e * T::get(v[r]);
+                }
+        }
     }
+    l = halves(l);
     if (!live) return;
     const long long at = (long long)(t.first + token) * p.q.heads + head;
     if (plan.splits > 1) {

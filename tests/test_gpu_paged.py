@@ -196,13 +196,41 @@ def test_keys_behind_a_window_may_be_anything(device):
 
 
 def test_infinite_scores_and_values(device):
-    """A NaN key reaches the rows that see it and no others; an infinite value too."""
+    """A NaN key reaches the rows that see it and no others."""
     s = make_step([(3, 40), (1, 40)], 4, 1, 64, 16, torch.bfloat16, device)
     page, slot = int(s["block_table"][0, 37 // 16]), 37 % 16
     clean = call(s)
     s["k_pages"][page, slot] = math.nan
     out = call(s)
     assert torch.isnan(out[:3]).all() and torch.equal(out[3], clean[3])
+
+
+@pytest.mark.parametrize("new,heads", [(3, (8, 2, 64)), (2, (4, 1, 256)), (100, (8, 2, 128)), (70, (4, 4, 64)), (40, (4, 1, 256))])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("window", [0, 20])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(device, window, dtype, new, heads):
+    """Infinities and NaN in the values of some of the step's own keys: rows before such a key, or past its window, are what they are
+    without it; rows that see it get the infinity or NaN, in the columns that hold one."""
+    total = new + 37
+    s = make_step([(new, total)], *heads, 16, dtype, device, seed=new)
+    clean, tol = exact_attention(s, window=window)
+    put = {total - 1: (5, math.inf), total - 2: (5, -math.inf), total - new: (7, math.nan), total - new // 2: (9, -math.inf), 3: (2, math.inf)}
+    for key, (d, x) in put.items():
+        s["v_pages"][int(s["block_table"][0, key // 16]), key % 16, :, d] = x
+    got = call(s, window=window).double().cpu()
+    want = clean.clone()
+    for i in range(new):
+        pos = total - new + i
+        sees = [key <= pos and (not window or key > pos - window) for key in put]
+        add = {}
+        for (key, (d, x)), see in zip(put.items(), sees):
+            if see:
+                add[d] = add.get(d, 0.0) + x
+        for d, x in add.items():
+            want[i, :, d] = x
+    odd = ~torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[odd].nan_to_num(1.0), want[odd].nan_to_num(1.0))
+    assert ((got[~odd] - want[~odd]).abs() <= tol[~odd]).all()
 
 
 def test_rows_behind_the_last_sequence_stay(device):
