@@ -134,6 +134,7 @@ constexpr int kFewSlots = 512;
 // Keys of a split of the few-rows kernel: what gives the card's workgroups equal shares of all sequences' keys, whose number only the
 // device knows. Asked by whole waves.
 __device__ __forceinline__ int few_least(const AttentionParams& p) {
+    if (p.step.seqs == 1) return kFewLeast;  // the splits share it out as it is
     long long keys = 0;
     for (int b = threadIdx.x & 63; b < p.step.seqs; b += 64) {
         const int n = min(max(p.step.lengths[b], 0), p.step.blocks * p.step.page_size);
@@ -814,15 +815,23 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttentionParams p, Att
     const float f = mine.y == 0.0f || mine.x == kNone ? 0.0f : __builtin_amdgcn_exp2f(mine.x - mx);
     const float sum = wave_sum(f * mine.y);
     const unsigned long long used = __ballot(mine.y != 0.0f);
+    const int n = used ? 64 - __builtin_clzll(used) : 0;  // splits that saw nothing come last, as a rule
     float o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
-    const float* part = plan.part + at * plan.splits * D;
-    for (unsigned long long left = used; left; left &= left - 1) {
-        const int i = __builtin_ctzll(left);
-        const float w = __shfl(f, i);
+    const float* part = plan.part + at * plan.splits * D + E * lane;
+    for (int i = 0; i < n; i += 4) {  // four at a time are on their way
+        float v[4][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += w * part[(long long)i * D + E * lane + e];
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[u][e] = part[(long long)min(i + u, n - 1) * D + e];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float w = i + u < n ? __shfl(f, i + u) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = w != 0.0f ? o[e] + w * v[u][e] : o[e];  // what a split that saw nothing holds is never read as a number
+        }
     }
     const float k = row_scale<M>(p, head, mx, sum);
     raw* out = static_cast<raw*>(p.out) + at * D + E * lane;
@@ -835,7 +844,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttentionParams p, Att
 bool attention_dim_ok(int dim) { return dim == 64 || dim == 128 || dim == 256; }
 
 constexpr int kMostSplits = 64;  // the join kernel holds a split's statistics per lane
-constexpr int kFewMost = 32;     // rows of a sequence that the few-rows kernel takes in one pass over its keys
+// Rows of a sequence that the few-rows kernel takes in one pass over its keys: two sets of 16, one where their registers would not do.
+static int few_most(int dim) { return dim <= 128 ? 32 : 16; }
 
 struct Forms {
     bool few, tile;
@@ -850,10 +860,11 @@ static Forms attention_forms(const AttentionParams& p) {
     const int even = (p.step.tokens + p.step.seqs - 1) / p.step.seqs;  // some sequence has at least that many tokens
     Forms f{};
     f.most = (long long)(p.max_new > p.step.tokens ? p.step.tokens : p.max_new < even ? even : p.max_new) * group;
-    f.tile = f.most > kFewMost;
+    const int few = few_most(p.dim);
+    f.tile = f.most > few;
     f.few = !f.tile || p.step.seqs > 1;
     // many-row sequences: at most one partly filled tile each
-    const long long seqs = p.step.seqs < rows / (kFewMost + 1) ? p.step.seqs : rows / (kFewMost + 1);
+    const long long seqs = p.step.seqs < rows / (few + 1) ? p.step.seqs : rows / (few + 1);
     f.tiles = f.tile ? (int)((rows + kTileRows - 1) / kTileRows + seqs) : 0;
     const long long groups = f.tile ? (long long)f.tiles * p.kv_heads : (long long)p.step.seqs * p.kv_heads;
     const long long want = ((f.tile ? 512 : f.most > 16 ? 2048 : 4096) + groups / 2) / groups;
@@ -872,7 +883,7 @@ size_t attention_workspace_bytes(const AttentionParams& p) {
 template <class M, int D>
 static hipError_t attention_d(const AttentionParams& p, hipStream_t s) {
     const Forms f = attention_forms(p);
-    AttentionPlan plan{f.splits, f.tile ? kFewMost : 0, p.ws};
+    AttentionPlan plan{f.splits, f.tile ? few_most(D) : 0, p.ws};
     if (f.tile) {
         const int lds = 4 * TileSize<D>::kBytes;
         if (!f.few) plan.few_rows = 0;
@@ -882,8 +893,8 @@ static hipError_t attention_d(const AttentionParams& p, hipStream_t s) {
         // splits slowest: the workgroups of one split number spread over the XCDs, and those without keys come last
         const dim3 grid(p.kv_heads, p.step.seqs, f.splits);
         const int lds = kFewWaves * 4 * kFewKeys * D * 2;  // the rings; the results of 16 rows take half of it
-        if (f.most <= 16) hipLaunchKernelGGL((attend_few_kernel<M, D, 1>), grid, dim3(64 * kFewWaves), lds, s, p, plan);
-        else hipLaunchKernelGGL((attend_few_kernel<M, D, 2>), grid, dim3(64 * kFewWaves), lds, s, p, plan);
+        if (D > 128 || f.most <= 16) hipLaunchKernelGGL((attend_few_kernel<M, D, 1>), grid, dim3(64 * kFewWaves), lds, s, p, plan);
+        else hipLaunchKernelGGL((attend_few_kernel<M, D <= 128 ? D : 128, 2>), grid, dim3(64 * kFewWaves), lds, s, p, plan);
     }
     if (f.splits > 1) {
         const long long rows = (long long)p.step.tokens * p.q.heads;
