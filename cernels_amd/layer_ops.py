@@ -277,7 +277,8 @@ def _check_step(like, k_pages, v_pages, block_table, lengths, q_offsets, tokens,
     _require(isinstance(block_table, torch.Tensor) and block_table.device == dev and block_table.dtype == torch.int32
              and block_table.dim() == 2 and (block_table.stride(1) == 1 or block_table.size(1) <= 1),
              "block_table must be int32 [sequences, blocks] with contiguous rows on the step's device")
-    seqs = block_table.size(0)
+    seqs, blocks = block_table.shape
+    _require(seqs <= 1 or block_table.stride(0) >= blocks, "block_table's rows must not overlap")
     _require(isinstance(lengths, torch.Tensor) and lengths.device == dev and lengths.dtype == torch.int32
              and lengths.shape == (seqs,) and lengths.is_contiguous(), "lengths must be contiguous int32 [sequences] on the step's device")
     if q_offsets is None:
@@ -297,7 +298,7 @@ def _step_ok(like, k_pages, v_pages, block_table, lengths, q_offsets, tokens, di
             and k_pages.dtype is dt and v_pages.dtype is dt and k_pages.get_device() == dev and v_pages.get_device() == dev
             and k_pages.stride(3) == 1 and v_pages.stride(3) == 1 and pages >= 1 and page_size >= 16 and page_size % 16 == 0
             and block_table.dtype is torch.int32 and block_table.get_device() == dev and (block_table.stride(1) == 1 or blocks <= 1)
-            and lengths.dtype is torch.int32 and lengths.get_device() == dev and lengths.shape == (seqs,) and lengths.is_contiguous()
+            and (block_table.stride(0) >= blocks or seqs <= 1) and lengths.dtype is torch.int32 and lengths.get_device() == dev and lengths.shape == (seqs,) and lengths.is_contiguous()
             and (tokens % max(seqs, 1) == 0 if q_offsets is None else
                  (q_offsets.dtype is torch.int32 and q_offsets.get_device() == dev and q_offsets.shape == (seqs + 1,)
                   and q_offsets.is_contiguous())))
@@ -362,7 +363,13 @@ def _check_attention(q, k_pages, v_pages, block_table, lengths, q_offsets, sinks
 
 
 def _pages_args(k_pages, v_pages):
-    return _Strides(*k_pages.stride()[:3], *v_pages.stride()[:3]), k_pages.size(0), k_pages.size(1)
+    pages, page_size, heads, _ = k_pages.shape
+    strides = _Strides(*k_pages.stride()[:3], *v_pages.stride()[:3])
+    if heads == 1:  # a stride that is never taken may be anything
+        strides[2] = strides[5] = 0
+    if pages == 1:
+        strides[0] = strides[3] = 0
+    return strides, pages, page_size
 
 
 def _table_args(block_table, lengths):
@@ -412,7 +419,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _refuse_gradient("paged_attention", q, k_pages, v_pages, sinks)
     tokens, heads, dim = q.shape
     kv_heads = k_pages.size(2)
-    _require(window >= 0, "window must not be negative")
+    _require(0 <= window < 2 ** 31, "window must be 0 (none) or a number of keys under 2^31")
     scale = dim ** -0.5 if scale is None else float(scale)
     _require(0.0 < scale < math.inf, "scale must be positive")
     if out is None:

@@ -150,8 +150,8 @@ class PagedDecoder:
         prompts = [p.reshape(-1) for p in prompts]
         longest = max(int(p.numel()) for p in prompts)
         size = longest if chunk is None else int(chunk)
-        if size < 1 or min(int(p.numel()) for p in prompts) < 1:
-            raise RuntimeError("prompts and chunks must hold at least one token")
+        if n < 1 or size < 1 or min(int(p.numel()) for p in prompts) < 1:
+            raise RuntimeError("prompts, chunks and continuations must hold at least one token")
         last = None
         for at in range(0, longest, size):
             logits = self.step([p[at:at + size] for p in prompts])

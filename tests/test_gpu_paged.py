@@ -168,6 +168,56 @@ def test_pages_in_other_orders(device, new):
     check(s, call(s))
 
 
+def test_strides_of_single_heads_and_pages_do_not_matter(device):
+    s = make_step([(1, 16)], 4, 1, 64, 16, torch.bfloat16, device)
+    page = int(s["block_table"][0, 0])
+    want = call(s)
+    k, v = (s[n][page:page + 1].contiguous().as_strided((1, 16, 1, 64), (3, 64, 5, 1)) for n in ("k_pages", "v_pages"))
+    got = ops.paged_attention(s["q"], k, v, torch.zeros_like(s["block_table"]), s["lengths"], s["q_offsets"])
+    assert torch.equal(got, want)
+
+
+def test_refusals(device):
+    """What breaks the contract is refused before a launch, on the GPU's own tensors."""
+    s = make_step([(2, 40), (1, 5)], 8, 2, 64, 16, torch.bfloat16, device, fill=0.0)
+    bad = [dict(q=s["q"].float()), dict(q=s["q"][..., :32]), dict(q=s["q"][:, :7]), dict(q=s["q"].cpu()), dict(lengths=s["lengths"].long()),
+           dict(lengths=s["lengths"][:1]), dict(q_offsets=s["q_offsets"][:2]), dict(block_table=s["block_table"].long()),
+           dict(block_table=s["block_table"][:1].expand(2, -1)), dict(block_table=s["block_table"].cpu()),
+           dict(k_pages=s["k_pages"][:, :8]), dict(k_pages=s["k_pages"].half()), dict(v_pages=s["v_pages"][:1]),
+           dict(k_pages=s["k_pages"].transpose(2, 3)), dict(q_offsets=None)]
+    for change in bad:
+        with pytest.raises(RuntimeError):
+            call({**s, **change}, q_offsets=change.get("q_offsets", s["q_offsets"]))
+        t = {**s, **change}
+        if t["q"] is not s["q"]:
+            continue
+        with pytest.raises(RuntimeError):
+            ops.paged_append(s["q"][:, :2], s["q"][:, :2], t["k_pages"], t["v_pages"], t["block_table"], t["lengths"], t["q_offsets"])
+    for kw in (dict(window=-1), dict(window=2 ** 32 + 5), dict(scale=0.0), dict(scale=math.nan), dict(sinks=torch.zeros(4, device=device)),
+               dict(sinks=torch.zeros(8, device=device, dtype=torch.bfloat16)), dict(out=s["q"][:, :4]), dict(max_new=-1)):
+        with pytest.raises(RuntimeError):
+            call(s, **kw)
+    off = torch.empty(s["k_pages"].numel() + 4, dtype=torch.bfloat16, device=device)[4:].view_as(s["k_pages"])
+    with pytest.raises(RuntimeError, match="aligned"):
+        call({**s, "k_pages": off})
+    inv = torch.ones(33, device=device)
+    for f in (inv, inv[:32].half(), inv[:32].cpu(), inv[:20][::2]):
+        with pytest.raises(RuntimeError):
+            ops.paged_append(s["q"][:, :2], s["q"][:, :2], s["k_pages"], s["v_pages"], s["block_table"], s["lengths"], s["q_offsets"], inv_freq=f)
+    with torch.enable_grad(), pytest.raises(RuntimeError, match="backward"):
+        call({**s, "q": s["q"].clone().requires_grad_()})
+    x = torch.zeros(4, 8, device=device)
+    for args in ((x.t(), torch.ones(4, device=device)), (x, torch.ones(7, device=device)), (x, torch.ones(8)), (x.double(), torch.ones(8, device=device)),
+                 (x, torch.ones(8, device=device).half()), (x, torch.ones(8, device=device), torch.ones(8, device=device).half())):
+        with pytest.raises(RuntimeError):
+            ops.layer_norm(*args)
+    q, pos, f = torch.zeros(4, 2, 8, device=device), torch.arange(4, device=device), torch.ones(4, device=device)
+    for args in ((q, None, pos[:3], f), (q, None, pos.float(), f), (q, q[:3], pos, f), (q, q.half(), pos, f), (q, None, pos, torch.ones(5, device=device)),
+                 (q.transpose(1, 2), None, pos, f), (q[0], None, pos, f), (q, None, pos.cpu(), f)):
+        with pytest.raises(RuntimeError):
+            ops.rotary(*args)
+
+
 @pytest.mark.parametrize("new", [1, 50])
 @pytest.mark.parametrize("fill", [math.nan, math.inf])
 def test_stale_slots_and_missing_pages(device, new, fill):
