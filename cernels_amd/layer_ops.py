@@ -37,6 +37,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _dense_like(t):
+    """A new contiguous tensor of t's shape, type and device, whatever t's strides."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -220,7 +225,7 @@ def _rotary_ok(q, k, positions, inv_freq) -> bool:
 def _rotary_launch(q, k, positions, inv_freq, interleaved, scale, backward):
     first = q if q is not None else k
     tokens, _, dim = first.shape
-    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    outs = [None if t is None else _dense_like(t) for t in (q, k)]
     if tokens:
         heads = [(None, 0, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1), t.size(1)) for t in (q, k)]
         _launch("cernels_rotary", first.get_device(), _native.lib().cernels_rotary, *heads[0], *heads[1], positions.data_ptr(),
@@ -392,7 +397,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     pairs = freq = 0
     if inv_freq is not None:
         pairs, freq = inv_freq.numel(), _FREQ_DTYPES[inv_freq.dtype]
-    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = None if q is None else _dense_like(q)
     seqs = block_table.size(0)
     if tokens and seqs:
         head = (None, 0, 0, 0) if q is None else (q.data_ptr(), q.stride(0), q.stride(1), q.size(1))
@@ -423,7 +428,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     scale = dim ** -0.5 if scale is None else float(scale)
     _require(0.0 < scale < math.inf, "scale must be positive")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        out = _dense_like(q)
     seqs, blocks, page_size = block_table.size(0), block_table.size(1), k_pages.size(1)
     if tokens and seqs:
         L = _native.lib()
