@@ -92,8 +92,8 @@ __device__ __forceinline__ void raise_to(float x, float& m, float& f, float& e) 
 
 // What a launch works on beside the call's own parameters.
 struct AttentionPlan {
-    int splits;    // workgroups that share a tile's keys; above 1 they write partial results
-    int few_rows;  // sequences of at most this many rows take the few-rows kernel, the others the tile kernel; 0: none takes it
+    int splits;    // parts that a sequence's keys may be cut in; above 1 workgroups write partial results
+    int few_rows;  // sequences of at most this many rows take the few-rows kernel, the others the tile kernel; -1: all take the former
     float* part;   // [tokens * heads][splits][dim] unnormalised O, then [tokens * heads][splits][2] M and sum
 };
 
@@ -101,15 +101,104 @@ __device__ __forceinline__ float2* plan_stats(const AttentionPlan& a, const Atte
     return reinterpret_cast<float2*>(a.part + (long long)p.step.tokens * p.q.heads * a.splits * p.dim);
 }
 
-// The part of the keys [begin, end) that split number `i` of `n` takes: whole multiples of `unit`, at least `least` keys a split.
-__device__ __forceinline__ void split_range(int begin, int end, int i, int n, int unit, int least, int& lo, int& hi) {
+// Part number `i` of `n` of the keys [begin, end): equal parts, whole multiples of `unit`.
+__device__ __forceinline__ void split_range(int begin, int end, int i, int n, int unit, int& lo, int& hi) {
     const int keys = end > begin ? end - begin : 0;
-    int per = (keys + n - 1) / n;
-    per = per < least ? least : per;
-    per = (per + unit - 1) / unit * unit;
+    const int per = max(((keys + n - 1) / n + unit - 1) / unit * unit, unit);
     const long long at = (long long)per * i;
     lo = at < keys ? begin + (int)at : end;
     hi = end - lo < per ? end : lo + per;
+}
+
+constexpr int kTileRows = 128;  // of the tile kernel
+constexpr int kSlots = 512;     // workgroups that are on the card at once: two per CU
+constexpr int kLeastKeys = 256;
+
+// A workgroup's work: one tile of rows of a sequence (all its rows: the few-rows kernel), and one of `parts` parts of their keys.
+struct Piece {
+    int b, first, count, rows, tile, split, parts;
+};
+// Piece number `i`, asked by whole waves; false behind the last one. Only the device knows the sequences' lengths, so the pieces are
+// listed by every workgroup for itself: a sequence's keys are cut so that the card's slots get equal shares of all of them, of 256
+// keys at least, and workgroups without a piece (which would hold a slot for some microseconds) are at most one per tile.
+template <bool FEW>
+__device__ __forceinline__ bool find_piece(const AttentionParams& p, const AttentionPlan& plan, int i, Piece& t) {
+    const int lane = threadIdx.x & 63, group = p.q.heads / p.kv_heads;
+    int first = 0, count = 0, rows = 0, tiles = 0, keys = 0;
+    auto look = [&](int b) __attribute__((always_inline)) {
+        first = count = tiles = keys = 0;
+        if (b < p.step.seqs) {
+            step_tokens(p.step, b, first, count);
+            const int length = p.step.lengths[b];
+            keys = min(max(length, 0), p.step.blocks * p.step.page_size);
+            if (p.window > 0) keys = (int)min((long long)keys, (long long)p.window + count);
+        }
+        rows = count * group;
+        const bool few = plan.few_rows < 0 || rows <= plan.few_rows;
+        tiles = rows == 0 || few != FEW ? 0 : FEW ? 1 : (rows + kTileRows - 1) / kTileRows;
+    };
+    auto cut = [&](float share) __attribute__((always_inline)) {
+        return min(max((int)ceilf((float)keys / share - 0.05f), 1), plan.splits);  // a twentieth over a share is no part of its own
+    };
+    if (p.step.seqs == 1) {  // no list: the same in all lanes
+        look(0);
+        t.parts = cut(fmaxf((float)tiles * (float)keys * (float)p.kv_heads * (1.0f / kSlots), (float)kLeastKeys));
+        if (tiles * p.kv_heads * t.parts > kSlots && t.parts > 1) t.parts = max(kSlots / (tiles * p.kv_heads), 1);
+        t.b = 0, t.first = first, t.count = count, t.rows = rows;
+        const int from_end = tiles * t.parts - 1 - i;
+        t.tile = from_end / t.parts;
+        t.split = from_end - t.tile * t.parts;
+        return from_end >= 0;
+    }
+    look(lane);
+    float share = 3.0e9f;
+    if (plan.splits > 1) {
+        float sum = 0.0f;
+        for (int b = lane;;) {
+            sum += (float)tiles * (float)keys;
+            b += 64;
+            if (b - lane >= p.step.seqs) break;
+            look(b);
+        }
+        share = fmaxf(wave_sum(sum) * (float)p.kv_heads * (1.0f / kSlots), (float)kLeastKeys);
+        if (p.step.seqs > 64) {
+            look(lane);
+        } else {  // equal sequences cut just over their share would be more pieces than slots, all of one size: a round more
+            const float pieces = wave_sum((float)(tiles * cut(share))) * (float)p.kv_heads;
+            if (pieces > kSlots) share *= fminf(pieces * (1.0f / kSlots), 1.5f);
+        }
+    }
+    for (int b0 = 0; b0 < p.step.seqs; b0 += 64) {
+        if (b0) look(b0 + lane);
+        const int parts = cut(share);
+        int sum = tiles * parts;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(sum, o);
+            if (lane >= o) sum += up;
+        }
+        const unsigned long long has = __ballot(sum > i);
+        if (has) {
+            const int l = __builtin_ctzll(has);
+            t.b = b0 + l;
+            t.first = __builtin_amdgcn_readlane(first, l);
+            t.count = __builtin_amdgcn_readlane(count, l);
+            t.rows = __builtin_amdgcn_readlane(rows, l);
+            t.parts = __builtin_amdgcn_readlane(parts, l);
+            const int from_end = __builtin_amdgcn_readlane(sum, l) - 1 - i;
+            t.tile = from_end / t.parts;  // the last tile first: it sees the most keys
+            t.split = from_end - t.tile * t.parts;
+            return true;
+        }
+        i -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
+// The splits that a sequence's parts leave unused saw nothing; the join reads that. Written by the workgroup of the first part.
+__device__ __forceinline__ void unused_splits(const AttentionParams& p, const AttentionPlan& plan, const Piece& t, long long row) {
+    if (t.split == 0)
+        for (int i = t.parts; i < plan.splits; ++i) plan_stats(plan, p)[row * plan.splits + i] = make_float2(kNone, 0.0f);
 }
 
 // One row's result: normalised into the output, or as a partial result of its split.
@@ -128,22 +217,6 @@ __device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
 // (ds_read_b64_tr_b16: 4 keys of one column per lane).
 constexpr int kFewWaves = 4;
 constexpr int kFewKeys = 16;
-constexpr int kFewLeast = 256;  // keys of a split
-constexpr int kFewSlots = 512;
-
-// Keys of a split of the few-rows kernel: what gives the card's workgroups equal shares of all sequences' keys, whose number only the
-// device knows. Asked by whole waves.
-__device__ __forceinline__ int few_least(const AttentionParams& p) {
-    if (p.step.seqs == 1) return kFewLeast;  // the splits share it out as it is
-    long long keys = 0;
-    for (int b = threadIdx.x & 63; b < p.step.seqs; b += 64) {
-        const int n = min(max(p.step.lengths[b], 0), p.step.blocks * p.step.page_size);
-        keys += p.window > 0 ? min(n, p.window) : n;
-    }
-    const float sum = wave_sum((float)keys) * (float)p.kv_heads;
-    return __builtin_amdgcn_readfirstlane(max(kFewLeast, (int)fminf(sum / kFewSlots, 1.0e9f)));
-}
-
 template <class M, int D, int NT>
 __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionParams p, AttentionPlan plan) {
     typedef typename M::T T;
@@ -159,18 +232,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
     __shared__ float2 lds_ml[kFewWaves][16];
     float* lds_o = reinterpret_cast<float*>(lds);  // [wave][16 * D]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const int b = blockIdx.y, kh = blockIdx.x, split = blockIdx.z;
-    const int group = p.q.heads / p.kv_heads;
-    int first, count;
-    step_tokens(p.step, b, first, count);
-    const int rows = count * group;
-    if (rows == 0 || (plan.few_rows > 0 && rows > plan.few_rows)) return;
+    const int kh = blockIdx.x % p.kv_heads, group = p.q.heads / p.kv_heads;
+    Piece t;
+    if (!find_piece<true>(p, plan, blockIdx.x / p.kv_heads, t)) return;
+    const int b = t.b, first = t.first, count = t.count, rows = t.rows, split = t.split;
     const int length = p.step.lengths[b], page_size = p.step.page_size;
     const char* kbase = static_cast<const char*>(p.k.p) + 2 * kh * p.k.head;
     const char* vbase = static_cast<const char*>(p.v.p) + 2 * kh * p.v.head;
     const auto* table = (const __attribute__((address_space(4))) int32_t*)(p.step.table + b * p.step.table_stride);
     const float c = p.scale * kLog2e;
-    const int least = plan.splits > 1 ? few_least(p) : 0;
     // from a copy's first row: this lane's row, and the vector that belongs at its place
     const int crow = lane / CH, cpos = lane % CH;
     uint32_t koff[kCopies], voff[kCopies];
@@ -224,7 +294,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
         all_hi = __builtin_amdgcn_readfirstlane(all_hi);
         all_lo = __builtin_amdgcn_readfirstlane(all_lo);
         int begin, end;
-        split_range(least_lo & ~(kFewKeys - 1), most_hi, split, plan.splits, kFewKeys * kFewWaves, least, begin, end);
+        split_range(least_lo & ~(kFewKeys - 1), most_hi, split, t.parts, kFewKeys * kFewWaves, begin, end);
         // this wave's quarter of them; a stage lies inside one page (pages hold a multiple of 16 slots), and the pages are walked along
         // the table without a division
         const int quarter = (end - begin + kFewKeys * kFewWaves - 1) / (kFewKeys * kFewWaves) * kFewKeys;
@@ -439,7 +509,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
                         *reinterpret_cast<u32x2*>(static_cast<raw*>(p.out) + at * D + d) =
                             u32x2{M::pack2(v[0] * k, v[1] * k), M::pack2(v[2] * k, v[3] * k)};
                 }
-                if (plan.splits > 1 && part == 0) plan_stats(plan, p)[at * plan.splits + split] = make_float2(mx, sum);
+                if (plan.splits > 1 && part == 0) {
+                    plan_stats(plan, p)[at * plan.splits + split] = make_float2(mx, sum);
+                    unused_splits(p, plan, t, at);
+                }
             }
         }
     }
@@ -450,46 +523,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
 // while one is worked on. K's 16-byte vectors are read as operands as they are; V's operands are columns, which LDS hands out turned
 // (ds_read_b64_tr_b16: 4 keys of one column per lane).
 constexpr int kTileWaves = 4;
-constexpr int kTileRows = 32 * kTileWaves;
+static_assert(kTileRows == 32 * kTileWaves, "a wave has 32 rows");
 
 template <int D>
 struct TileSize {
     static constexpr int kKeys = D <= 128 ? 64 : 32;
     static constexpr int kBytes = kKeys * D * 2;
 };
-
-// Which tile of which sequence workgroup `i` has: tiles are numbered over the sequences with more than few_rows rows.
-struct TileId {
-    int b, row0, rows, first, count;
-};
-__device__ __forceinline__ bool find_tile(const AttentionParams& p, const AttentionPlan& plan, int i, TileId& t) {
-    const int lane = threadIdx.x & 63, group = p.q.heads / p.kv_heads;
-    for (int b0 = 0; b0 < p.step.seqs; b0 += 64) {
-        const int b = b0 + lane;
-        int first = 0, count = 0;
-        if (b < p.step.seqs) step_tokens(p.step, b, first, count);
-        const int rows = count * group;
-        const int tiles = rows > plan.few_rows ? (rows + kTileRows - 1) / kTileRows : 0;
-        int sum = tiles;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(sum, o);
-            if (lane >= o) sum += up;
-        }
-        const unsigned long long has = __ballot(sum > i);
-        if (has) {
-            const int l = __builtin_ctzll(has);
-            t.b = b0 + l;
-            t.first = __builtin_amdgcn_readlane(first, l);
-            t.count = __builtin_amdgcn_readlane(count, l);
-            t.rows = __builtin_amdgcn_readlane(rows, l);
-            t.row0 = (__builtin_amdgcn_readlane(sum, l) - 1 - i) * kTileRows;  // the last tile first: it sees the most keys
-            return true;
-        }
-        i -= __builtin_amdgcn_readlane(sum, 63);
-    }
-    return false;
-}
 
 template <class M, int D>
 __global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile_kernel(AttentionParams p, AttentionPlan plan) {
@@ -506,14 +546,15 @@ __global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile
     __shared__ __align__(16) uint32_t missing[4][kTileWaves];  // per tile and wave's run of keys: without a page
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int kh = blockIdx.x % p.kv_heads, group = p.q.heads / p.kv_heads;
-    TileId t;
-    if (!find_tile(p, plan, blockIdx.x / p.kv_heads, t)) return;
+    Piece t;
+    if (!find_piece<false>(p, plan, blockIdx.x / p.kv_heads, t)) return;
+    const int row0 = t.tile * kTileRows;
     const int length = p.step.lengths[t.b];
     const char* kbase = static_cast<const char*>(p.k.p) + 2 * kh * p.k.head;
     const char* vbase = static_cast<const char*>(p.v.p) + 2 * kh * p.v.head;
     const float c = p.scale * kLog2e;
 
-    const int row = t.row0 + 32 * wave + col;
+    const int row = row0 + 32 * wave + col;
     const bool live = row < t.rows;
     const int token = live ? row / group : 0, head = kh * group + (live ? row - token * group : 0);
     u32x4 q[DS];
@@ -526,13 +567,13 @@ __global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile
     const int page_size = p.step.page_size, cap = p.step.blocks * page_size, before = length - t.count;
     auto low = [&](int tok) __attribute__((always_inline)) { return p.window > 0 && before + tok - p.window + 1 > 0 ? before + tok - p.window + 1 : 0; };
     const int hi = live ? before + token + 1 : 0, lo = low(token);
-    const int last_row = min(t.row0 + kTileRows, t.rows) - 1;
-    const int w_first = min(t.row0 + 32 * wave, last_row) / group, w_last = min(t.row0 + 32 * wave + 31, last_row) / group;
-    bool idle = t.row0 + 32 * wave >= t.rows;
+    const int last_row = min(row0 + kTileRows, t.rows) - 1;
+    const int w_first = min(row0 + 32 * wave, last_row) / group, w_last = min(row0 + 32 * wave + 31, last_row) / group;
+    bool idle = row0 + 32 * wave >= t.rows;
     const int w_hi = before + w_last + 1, w_all_hi = before + w_first + 1, w_lo = low(w_first), w_all_lo = low(w_last);
-    const int tile_lo = low(t.row0 / group);
+    const int tile_lo = low(row0 / group);
     int begin, end;
-    split_range(tile_lo / KT * KT, min(before + last_row / group + 1, cap), blockIdx.y, plan.splits, KT, 4 * KT, begin, end);
+    split_range(tile_lo / KT * KT, min(before + last_row / group + 1, cap), t.split, t.parts, KT, begin, end);
 
     // This wave's run of the next tile to copy: its page and first slot, walked along the table without a division. Keys are sent one
     // tile ahead of the values, so the values' run is the one that the keys had before.
@@ -777,8 +818,11 @@ __global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile
     if (!live) return;
     const long long at = (long long)(t.first + token) * p.q.heads + head;
     if (plan.splits > 1) {
-        if (h == 0) plan_stats(plan, p)[at * plan.splits + blockIdx.y] = make_float2(m, l);
-        float* part = plan.part + (at * plan.splits + blockIdx.y) * D;
+        if (h == 0) {
+            plan_stats(plan, p)[at * plan.splits + t.split] = make_float2(m, l);
+            unused_splits(p, plan, t, at);
+        }
+        float* part = plan.part + (at * plan.splits + t.split) * D;
         if (l == 0.0f) return;  // nobody reads it
 #pragma unroll
         for (int j = 0; j < DT; ++j)
@@ -844,33 +888,37 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttentionParams p, Att
 bool attention_dim_ok(int dim) { return dim == 64 || dim == 128 || dim == 256; }
 
 constexpr int kMostSplits = 64;  // the join kernel holds a split's statistics per lane
-// Rows of a sequence that the few-rows kernel takes in one pass over its keys: two sets of 16, one where their registers would not do.
-static int few_most(int dim) { return dim <= 128 ? 32 : 16; }
+// Rows of a sequence that take the few-rows kernel: one set of 16.
+constexpr int kFewRows = 16;
 
 struct Forms {
     bool few, tile;
-    int splits, tiles;
-    long long most;  // rows of the sequence with the most of them, as far as the caller says
+    int splits;
+    long long few_pieces, tile_pieces;  // at most, for each key head
 };
 
 static Forms attention_forms(const AttentionParams& p) {
-    const int group = p.q.heads / p.kv_heads;
+    const int group = p.q.heads / p.kv_heads, seqs = p.step.seqs;
     const long long rows = (long long)p.step.tokens * group;
-    const long long keys = (long long)p.step.blocks * p.step.page_size;
-    const int even = (p.step.tokens + p.step.seqs - 1) / p.step.seqs;  // some sequence has at least that many tokens
+    const int even = (p.step.tokens + seqs - 1) / seqs;  // some sequence has at least that many tokens
+    const long long most = (long long)(p.max_new > p.step.tokens ? p.step.tokens : p.max_new < even ? even : p.max_new) * group;
     Forms f{};
-    f.most = (long long)(p.max_new > p.step.tokens ? p.step.tokens : p.max_new < even ? even : p.max_new) * group;
-    const int few = few_most(p.dim);
-    f.tile = f.most > few;
-    f.few = !f.tile || p.step.seqs > 1;
+    f.tile = most > kFewRows;
+    // as many tokens as the longest sequence's for each: all are alike, and one kernel takes them all, whatever they hold in truth
+    f.few = !f.tile || most * seqs != rows;
     // many-row sequences: at most one partly filled tile each
-    const long long seqs = p.step.seqs < rows / (few + 1) ? p.step.seqs : rows / (few + 1);
-    f.tiles = f.tile ? (int)((rows + kTileRows - 1) / kTileRows + seqs) : 0;
-    const long long groups = f.tile ? (long long)f.tiles * p.kv_heads : (long long)p.step.seqs * p.kv_heads;
-    const long long want = ((f.tile ? 512 : f.most > 16 ? 2048 : 4096) + groups / 2) / groups;
-    const long long useful = (keys + 255) / 256;
+    const long long part = rows / (kFewRows + 1);
+    const long long tiles = f.tile ? (rows + kTileRows - 1) / kTileRows + (seqs == 1 ? 0 : seqs < part ? seqs : part) : 0;
+    // Room for partial results: one sequence's tiles are cut alike; among several a long one is cut in more parts than the average, up
+    // to twice as many (tiles) or eight times (sets of 16 rows).
+    const long long groups = (f.tile ? tiles : seqs) * p.kv_heads;
+    const long long want = seqs == 1 ? kSlots / groups : ((f.tile ? 2 * kSlots : 8 * kSlots) + groups / 2) / groups;
+    const long long useful = ((long long)p.step.blocks * p.step.page_size + kLeastKeys - 1) / kLeastKeys;
     const long long n = want < useful ? want : useful;
     f.splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+    const long long cuts = f.splits > 1 ? (kSlots + p.kv_heads - 1) / p.kv_heads : 0;
+    f.few_pieces = f.few ? seqs + cuts : 0;
+    f.tile_pieces = f.tile ? tiles + cuts : 0;
     return f;
 }
 
@@ -883,19 +931,13 @@ size_t attention_workspace_bytes(const AttentionParams& p) {
 template <class M, int D>
 static hipError_t attention_d(const AttentionParams& p, hipStream_t s) {
     const Forms f = attention_forms(p);
-    AttentionPlan plan{f.splits, f.tile ? few_most(D) : 0, p.ws};
-    if (f.tile) {
-        const int lds = 4 * TileSize<D>::kBytes;
-        if (!f.few) plan.few_rows = 0;
-        hipLaunchKernelGGL((attend_tile_kernel<M, D>), dim3(f.tiles * p.kv_heads, f.splits), dim3(64 * kTileWaves), lds, s, p, plan);
-    }
-    if (f.few) {
-        // splits slowest: the workgroups of one split number spread over the XCDs, and those without keys come last
-        const dim3 grid(p.kv_heads, p.step.seqs, f.splits);
-        const int lds = kFewWaves * 4 * kFewKeys * D * 2;  // the rings; the results of 16 rows take half of it
-        if (D > 128 || f.most <= 16) hipLaunchKernelGGL((attend_few_kernel<M, D, 1>), grid, dim3(64 * kFewWaves), lds, s, p, plan);
-        else hipLaunchKernelGGL((attend_few_kernel<M, D <= 128 ? D : 128, 2>), grid, dim3(64 * kFewWaves), lds, s, p, plan);
-    }
+    const AttentionPlan plan{f.splits, f.tile ? (f.few ? kFewRows : 0) : -1, p.ws};
+    if (f.tile)
+        hipLaunchKernelGGL((attend_tile_kernel<M, D>), dim3((unsigned)(f.tile_pieces * p.kv_heads)), dim3(64 * kTileWaves),
+                           4 * TileSize<D>::kBytes, s, p, plan);
+    if (f.few)  // the rings; the results of 16 rows take half of them
+        hipLaunchKernelGGL((attend_few_kernel<M, D, 1>), dim3((unsigned)(f.few_pieces * p.kv_heads)), dim3(64 * kFewWaves),
+                           kFewWaves * 4 * kFewKeys * D * 2, s, p, plan);
     if (f.splits > 1) {
         const long long rows = (long long)p.step.tokens * p.q.heads;
         hipLaunchKernelGGL((attend_join_kernel<M, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p, plan);
