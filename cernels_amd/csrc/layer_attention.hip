@@ -111,7 +111,8 @@ __device__ __forceinline__ void split_range(int begin, int end, int i, int n, in
 }
 
 constexpr int kTileRows = 128;  // of the tile kernel
-constexpr int kSlots = 512;     // workgroups that are on the card at once: two per CU
+// Workgroups that are on the card at once: as the rings in LDS (few rows) and the registers (tiles) let on a CU.
+constexpr int card_slots(bool few, int dim) { return few ? 65536 / dim : dim <= 128 ? 512 : 256; }
 constexpr int kLeastKeys = 256;
 
 // A workgroup's work: one tile of rows of a sequence (all its rows: the few-rows kernel), and one of `parts` parts of their keys.
@@ -121,8 +122,9 @@ struct Piece {
 // Piece number `i`, asked by whole waves; false behind the last one. Only the device knows the sequences' lengths, so the pieces are
 // listed by every workgroup for itself: a sequence's keys are cut so that the card's slots get equal shares of all of them, of 256
 // keys at least, and workgroups without a piece (which would hold a slot for some microseconds) are at most one per tile.
-template <bool FEW>
+template <bool FEW, int D>
 __device__ __forceinline__ bool find_piece(const AttentionParams& p, const AttentionPlan& plan, int i, Piece& t) {
+    constexpr int kSlots = card_slots(FEW, D);
     const int lane = threadIdx.x & 63, group = p.q.heads / p.kv_heads;
     int first = 0, count = 0, rows = 0, tiles = 0, keys = 0;
     auto look = [&](int b) __attribute__((always_inline)) {
@@ -217,7 +219,8 @@ __device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
 // (ds_read_b64_tr_b16: 4 keys of one column per lane).
 constexpr int kFewWaves = 4;
 constexpr int kFewKeys = 16;
-template <class M, int D, int NT>
+
+template <class M, int D>
 __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionParams p, AttentionPlan plan) {
     typedef typename M::T T;
     typedef typename T::raw raw;
@@ -234,7 +237,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int kh = blockIdx.x % p.kv_heads, group = p.q.heads / p.kv_heads;
     Piece t;
-    if (!find_piece<true>(p, plan, blockIdx.x / p.kv_heads, t)) return;
+    if (!find_piece<true, D>(p, plan, blockIdx.x / p.kv_heads, t)) return;
     const int b = t.b, first = t.first, count = t.count, rows = t.rows, split = t.split;
     const int length = p.step.lengths[b], page_size = p.step.page_size;
     const char* kbase = static_cast<const char*>(p.k.p) + 2 * kh * p.k.head;
@@ -260,27 +263,23 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
         vaddr[j] = ring + kBytes + r * D * 2 + 16 * (chunk ^ (2 * r & kMask)) + 8 * (lane & 1);
     }
 
-    for (int r0 = 0; r0 < rows; r0 += 16 * NT) {
-        // rows r0 .. r0 + 16 NT - 1: this lane's columns, their queries and the keys that they see
-        u32x4 q[NT][DS];
-        int hi[NT], lo[NT], most_hi = 0, least_lo = 0x7fffffff, all_hi = 0x7fffffff, all_lo = 0;
+    for (int r0 = 0; r0 < rows; r0 += 16) {
+        // rows r0 .. r0 + 15: this lane's, its query and the keys that they see
+        u32x4 q[DS];
+        int most_hi = 0, least_lo = 0x7fffffff, all_hi = 0x7fffffff, all_lo = 0;
+        const int row = r0 + col;
+        const bool live = row < rows;
+        const int token = live ? row / group : 0, head = kh * group + (live ? row - token * group : 0);
+        const raw* src = static_cast<const raw*>(p.q.p) + (first + token) * p.q.token + head * p.q.head;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int row = r0 + 16 * n + col;
-            const bool live = row < rows;
-            const int token = live ? row / group : 0, head = kh * group + (live ? row - token * group : 0);
-            const raw* src = static_cast<const raw*>(p.q.p) + (first + token) * p.q.token + head * p.q.head;
-#pragma unroll
-            for (int s = 0; s < DS; ++s) q[n][s] = live ? load_vec<T>(src + 8 * (g + 4 * s)) : u32x4{};
-            const int pos = length - count + token;
-            hi[n] = live ? pos + 1 : 0;
-            lo[n] = p.window > 0 && pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
-            if (live) {
-                most_hi = max(most_hi, hi[n]);
-                least_lo = min(least_lo, lo[n]);
-                all_hi = min(all_hi, hi[n]);
-                all_lo = max(all_lo, lo[n]);
-            }
+        for (int s = 0; s < DS; ++s) q[s] = live ? load_vec<T>(src + 8 * (g + 4 * s)) : u32x4{};
+        const int pos = length - count + token;
+        const int hi = live ? pos + 1 : 0, lo = p.window > 0 && pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
+        if (live) {
+            most_hi = max(most_hi, hi);
+            least_lo = min(least_lo, lo);
+            all_hi = min(all_hi, hi);
+            all_lo = max(all_lo, lo);
         }
 #pragma unroll
         for (int o = 8; o; o >>= 1) {
@@ -333,29 +332,21 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
             }
         };
 
-        float m[NT], l[NT];
-        f32x4 o[NT][DJ];
+        float m = kNone, l = 0.0f;
+        f32x4 o[DJ];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            m[n] = kNone;
-            l[n] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < DJ; ++j) o[n][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
+        for (int j = 0; j < DJ; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         // One stage: 16 keys from k0, `left` keys to come with them. K of the stage after next is sent once this stage's is read, V
         // likewise; a wait leaves in flight what was sent after what it waits for.
         auto step = [&](int k0, int left, bool bad, const Run& next, auto which) __attribute__((always_inline)) {
             constexpr int kBase = decltype(which)::value * 2 * kBytes;
             if (left > kFewKeys) wait_vmcnt<3 * kCopies>();
             else wait_vmcnt<kCopies>();
-            f32x4 s[NT];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) s[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            f32x4 s{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int d = 0; d < DS; ++d) {
                 const u32x4 a = *(lds_vec)(kaddr[d] + kBase);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) s[n] = M::mma16(a, q[n][d], s[n]);
+                s = M::mma16(a, q[d], s);
             }
             if ((k0 < all_lo || k0 + kFewKeys > all_hi)) {  // some row does not see some key
                 wait_vmcnt<0>();
@@ -367,44 +358,39 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
             const bool sent = left > 2 * kFewKeys;
             if (sent) copy_keys(next, decltype(which)::value);
             const bool whole = !bad && k0 >= all_lo && k0 + kFewKeys <= all_hi && left >= kFewKeys;
-            u32x2 pr[NT];
+            if (!whole) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (!whole) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = k0 + 4 * g + i;
-                        const bool sees = !bad & (key < hi[n]) & (key >= lo[n]) & (key < w_end);
-                        s[n][i] = sees ? s[n][i] : kNone;
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const int key = k0 + 4 * g + i;
+                    const bool sees = !bad & (key < hi) & (key >= lo) & (key < w_end);
+                    s[i] = sees ? s[i] : kNone;
                 }
-                float t = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])) * c;
-                if (__ballot(t > m[n] + kSlack) != 0) {
-                    t = fmaxf(t, __shfl_xor(t, 16));
-                    t = fmaxf(t, __shfl_xor(t, 32));
-                    const float m1 = fmaxf(m[n], t);
-                    const float f = m1 == kNone ? 1.0f : __builtin_amdgcn_exp2f(m[n] - m1);
-                    m[n] = m1;
-                    l[n] *= f;
-#pragma unroll
-                    for (int j = 0; j < DJ; ++j) o[n][j] *= f;
-                }
-                const float sub = m[n] == kNone ? 0.0f : m[n];
-                float e[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c, -sub));
-                // rounded to the values' type for the product; the sum takes the rounded ones too (as in the tile kernel)
-                pr[n] = u32x2{M::pack2(e[0], e[1]), M::pack2(e[2], e[3])};
-                l[n] = M::add2(pr[n][1], M::add2(pr[n][0], l[n]));
             }
+            float t = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) * c;
+            if (__ballot(t > m + kSlack) != 0) {
+                t = fmaxf(t, __shfl_xor(t, 16));
+                t = fmaxf(t, __shfl_xor(t, 32));
+                const float m1 = fmaxf(m, t);
+                const float f = m1 == kNone ? 1.0f : __builtin_amdgcn_exp2f(m - m1);
+                m = m1;
+                l *= f;
+#pragma unroll
+                for (int j = 0; j < DJ; ++j) o[j] *= f;
+            }
+            const float sub = m == kNone ? 0.0f : m;
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -sub));
+            // rounded to the values' type for the product; the sum takes the rounded ones too (as in the tile kernel)
+            const u32x2 pr{M::pack2(e[0], e[1]), M::pack2(e[2], e[3])};
+            l = M::add2(pr[1], M::add2(pr[0], l));
             if (sent) wait_vmcnt<3 * kCopies>();
             else if (left > kFewKeys) wait_vmcnt<2 * kCopies>();
             else wait_vmcnt<0>();
 #pragma unroll
             for (int j = 0; j < DJ; ++j) {
                 const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_turned)(vaddr[j] + kBase));
-#pragma unroll
-                for (int n = 0; n < NT; ++n) o[n][j] = M::mma16_short(a, pr[n], o[n][j]);
+                o[j] = M::mma16_short(a, pr, o[j]);
             }
             if (sent) copy_values(next, decltype(which)::value);
             return false;
@@ -450,69 +436,63 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
             if (at.page < 0) continue;
             const char* kp = kbase + 2 * ((long long)at.page * p.k.page + at.slot * p.k.slot);
             const char* vp = vbase + 2 * ((long long)at.page * p.v.page + at.slot * p.v.slot);
+            float x = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float x = 0.0f;
+            for (int d = 0; d < DS; ++d) x = dot8<T>(*reinterpret_cast<const u32x4*>(kp + 64 * d + 16 * g), q[d], x);
+            x += __shfl_xor(x, 16);
+            x = (x + __shfl_xor(x, 32)) * c;
+            if (key < hi && key >= lo) {
+                float f, e;
+                raise_to(x, m, f, e);
+                l = l * f + (g == 0 ? e : 0.0f);
 #pragma unroll
-                for (int d = 0; d < DS; ++d) x = dot8<T>(*reinterpret_cast<const u32x4*>(kp + 64 * d + 16 * g), q[n][d], x);
-                x += __shfl_xor(x, 16);
-                x = (x + __shfl_xor(x, 32)) * c;
-                if (key < hi[n] && key >= lo[n]) {
-                    float f, e;
-                    raise_to(x, m[n], f, e);
-                    l[n] = l[n] * f + (g == 0 ? e : 0.0f);
+                for (int j = 0; j < DJ; ++j)
 #pragma unroll
-                    for (int j = 0; j < DJ; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            o[n][j][i] = o[n][j][i] * f + e * T::get(reinterpret_cast<const raw*>(vp)[16 * j + 4 * g + i]);
-                }
+                    for (int i = 0; i < 4; ++i)
+                        o[j][i] = o[j][i] * f + e * T::get(reinterpret_cast<const raw*>(vp)[16 * j + 4 * g + i]);
             }
         }
-        // the waves' results, one set of 16 rows after the other
+        // the waves' results
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        __syncthreads();
+        if (g == 0) lds_ml[wave][col] = make_float2(m, l);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            l[n] += __shfl_xor(l[n], 16);
-            l[n] += __shfl_xor(l[n], 32);
-            __syncthreads();
-            if (g == 0) lds_ml[wave][col] = make_float2(m[n], l[n]);
+        for (int j = 0; j < DJ; ++j)
 #pragma unroll
-            for (int j = 0; j < DJ; ++j)
+            for (int r = 0; r < 4; ++r) {
+                const int d = 16 * j + 4 * g + r;
+                lds_o[wave * 16 * D + col * D + (d ^ (col & 7) * 4)] = o[j][r];
+            }
+        __syncthreads();
+        constexpr int kPer = 64 * kFewWaves / 16;  // threads that share a row
+        const int my = threadIdx.x / kPer, part = threadIdx.x % kPer, mine = r0 + my;
+        if (mine < rows) {
+            float mx = kNone, sum = 0.0f, f[kFewWaves];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = 16 * j + 4 * g + r;
-                    lds_o[wave * 16 * D + col * D + (d ^ (col & 7) * 4)] = o[n][j][r];
-                }
-            __syncthreads();
-            constexpr int kPer = 64 * kFewWaves / 16;  // threads that share a row
-            const int my = threadIdx.x / kPer, part = threadIdx.x % kPer, row = r0 + 16 * n + my;
-            if (row < rows) {
-                float mx = kNone, sum = 0.0f, f[kFewWaves];
+            for (int w = 0; w < kFewWaves; ++w) mx = fmaxf(mx, lds_ml[w][my].x);
 #pragma unroll
-                for (int w = 0; w < kFewWaves; ++w) mx = fmaxf(mx, lds_ml[w][my].x);
+            for (int w = 0; w < kFewWaves; ++w) {
+                f[w] = lds_ml[w][my].x == kNone ? 0.0f : __builtin_amdgcn_exp2f(lds_ml[w][my].x - mx);
+                sum += f[w] * lds_ml[w][my].y;
+            }
+            const int token = mine / group, head = kh * group + mine - token * group;
+            const long long at = (long long)(first + token) * p.q.heads + head;
+            const float k = plan.splits > 1 ? 1.0f : row_scale<M>(p, head, mx, sum);
+            for (int d = 4 * part; d < D; d += 4 * kPer) {
+                f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int w = 0; w < kFewWaves; ++w) {
-                    f[w] = lds_ml[w][my].x == kNone ? 0.0f : __builtin_amdgcn_exp2f(lds_ml[w][my].x - mx);
-                    sum += f[w] * lds_ml[w][my].y;
-                }
-                const int token = row / group, head = kh * group + row - token * group;
-                const long long at = (long long)(first + token) * p.q.heads + head;
-                const float k = plan.splits > 1 ? 1.0f : row_scale<M>(p, head, mx, sum);
-                for (int d = 4 * part; d < D; d += 4 * kPer) {
-                    f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int w = 0; w < kFewWaves; ++w)
-                        v += f[w] * *reinterpret_cast<const f32x4*>(&lds_o[w * 16 * D + my * D + (d ^ (my & 7) * 4)]);
-                    if (plan.splits > 1)
-                        *reinterpret_cast<f32x4*>(plan.part + (at * plan.splits + split) * D + d) = v;
-                    else
-                        *reinterpret_cast<u32x2*>(static_cast<raw*>(p.out) + at * D + d) =
-                            u32x2{M::pack2(v[0] * k, v[1] * k), M::pack2(v[2] * k, v[3] * k)};
-                }
-                if (plan.splits > 1 && part == 0) {
-                    plan_stats(plan, p)[at * plan.splits + split] = make_float2(mx, sum);
-                    unused_splits(p, plan, t, at);
-                }
+                for (int w = 0; w < kFewWaves; ++w)
+                    v += f[w] * *reinterpret_cast<const f32x4*>(&lds_o[w * 16 * D + my * D + (d ^ (my & 7) * 4)]);
+                if (plan.splits > 1)
+                    *reinterpret_cast<f32x4*>(plan.part + (at * plan.splits + split) * D + d) = v;
+                else
+                    *reinterpret_cast<u32x2*>(static_cast<raw*>(p.out) + at * D + d) =
+                        u32x2{M::pack2(v[0] * k, v[1] * k), M::pack2(v[2] * k, v[3] * k)};
+            }
+            if (plan.splits > 1 && part == 0) {
+                plan_stats(plan, p)[at * plan.splits + split] = make_float2(mx, sum);
+                unused_splits(p, plan, t, at);
             }
         }
     }
@@ -547,7 +527,7 @@ __global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const int kh = blockIdx.x % p.kv_heads, group = p.q.heads / p.kv_heads;
     Piece t;
-    if (!find_piece<false>(p, plan, blockIdx.x / p.kv_heads, t)) return;
+    if (!find_piece<false, D>(p, plan, blockIdx.x / p.kv_heads, t)) return;
     const int row0 = t.tile * kTileRows;
     const int length = p.step.lengths[t.b];
     const char* kbase = static_cast<const char*>(p.k.p) + 2 * kh * p.k.head;
@@ -912,13 +892,14 @@ static Forms attention_forms(const AttentionParams& p) {
     // Room for partial results: one sequence's tiles are cut alike; among several a long one is cut in more parts than the average, up
     // to twice as many (tiles) or eight times (sets of 16 rows).
     const long long groups = (f.tile ? tiles : seqs) * p.kv_heads;
-    const long long want = seqs == 1 ? kSlots / groups : ((f.tile ? 2 * kSlots : 8 * kSlots) + groups / 2) / groups;
+    const long long slots = card_slots(!f.tile, p.dim);
+    const long long want = seqs == 1 ? slots / groups : ((f.tile ? 2 : 8) * slots + groups / 2) / groups;
     const long long useful = ((long long)p.step.blocks * p.step.page_size + kLeastKeys - 1) / kLeastKeys;
     const long long n = want < useful ? want : useful;
     f.splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
-    const long long cuts = f.splits > 1 ? (kSlots + p.kv_heads - 1) / p.kv_heads : 0;
-    f.few_pieces = f.few ? seqs + cuts : 0;
-    f.tile_pieces = f.tile ? tiles + cuts : 0;
+    auto cuts = [&](bool few) { return f.splits > 1 ? (card_slots(few, p.dim) + p.kv_heads - 1) / p.kv_heads : 0; };
+    f.few_pieces = f.few ? seqs + cuts(true) : 0;
+    f.tile_pieces = f.tile ? tiles + cuts(false) : 0;
     return f;
 }
 
@@ -936,7 +917,7 @@ static hipError_t attention_d(const AttentionParams& p, hipStream_t s) {
         hipLaunchKernelGGL((attend_tile_kernel<M, D>), dim3((unsigned)(f.tile_pieces * p.kv_heads)), dim3(64 * kTileWaves),
                            4 * TileSize<D>::kBytes, s, p, plan);
     if (f.few)  // the rings; the results of 16 rows take half of them
-        hipLaunchKernelGGL((attend_few_kernel<M, D, 1>), dim3((unsigned)(f.few_pieces * p.kv_heads)), dim3(64 * kFewWaves),
+        hipLaunchKernelGGL((attend_few_kernel<M, D>), dim3((unsigned)(f.few_pieces * p.kv_heads)), dim3(64 * kFewWaves),
                            kFewWaves * 4 * kFewKeys * D * 2, s, p, plan);
     if (f.splits > 1) {
         const long long rows = (long long)p.step.tokens * p.q.heads;
