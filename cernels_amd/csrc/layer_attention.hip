@@ -8,6 +8,8 @@
 // holds are exactly the elements that it has to supply as the second operand of O^T = V^T P^T, once the keys of a tile are numbered in
 // the order in which the result registers hold them. The probabilities go from one product to the next without leaving the lane.
 //
+// Rows in sets of 16 (few) or 128 (tiles): see the two kernels. Launches: one or both of them, and a join where keys were split.
+//
 // M is raised only where a new score passes it by kSlack (a factor 2^kSlack in the exponentials, exact in fp32 and harmless in the
 // 16-bit probabilities), so that most tiles need neither a reduction over lanes nor a rescaling of O.
 #include "layer_step.h"
@@ -121,7 +123,8 @@ struct Piece {
 };
 // Piece number `i`, asked by whole waves; false behind the last one. Only the device knows the sequences' lengths, so the pieces are
 // listed by every workgroup for itself: a sequence's keys are cut so that the card's slots get equal shares of all of them, of 256
-// keys at least, and workgroups without a piece (which would hold a slot for some microseconds) are at most one per tile.
+// keys at least (128: 17 users with sinks 27.9 us, 256: 23.1), and workgroups without a piece, which hold a slot for some
+// microseconds, are at most one per tile (a grid of 16 splits for each of 64 sequences of 4096 keys: 136 us, the list: 111).
 template <bool FEW, int D>
 __device__ __forceinline__ bool find_piece(const AttentionParams& p, const AttentionPlan& plan, int i, Piece& t) {
     constexpr int kSlots = card_slots(FEW, D);
@@ -214,9 +217,12 @@ __device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
 
 // ---- few rows: single tokens and short chunks ---------------------------------------------------------------------------------
 // Bound by the stream of keys and values. The four waves of a workgroup share out its keys, and each runs alone: 16 keys at a time
-// come through a ring of two stages of its own in LDS, sent there without passing through registers, so that 16 to 32 KB per wave
-// are on their way at any time however few registers the products leave. Keys are read as operands as they lie, values turned
+// come through a ring of two stages of its own in LDS, sent there without passing through registers, so that a ring of 16 KB per
+// wave (heads of 128) is on its way at any time however few registers the products leave (keys and values taken straight into
+// operand registers: 64 users with mixed lengths 102 us, rings 87). Keys are read as operands as they lie, values turned
 // (ds_read_b64_tr_b16: 4 keys of one column per lane).
+// Measured: 64 users of 4096 keys (32 query, 4 key heads of 128) 111 us with the join, 4.8 TB/s, where a large copy moves 5.2; 64
+// users with 195 to 8193 keys 70 us, 3.8 TB/s; one user behind 2168 keys 9 us and the join's 4.5, bound by latency.
 constexpr int kFewWaves = 4;
 constexpr int kFewKeys = 16;
 
@@ -501,7 +507,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
 // ---- many rows: chunks and prompts --------------------------------------------------------------------------------------------
 // Bound by the matrix instructions. Four waves of 32 rows each share tiles of keys and values in LDS, the next tile on its way there
 // while one is worked on. K's 16-byte vectors are read as operands as they are; V's operands are columns, which LDS hands out turned
-// (ds_read_b64_tr_b16: 4 keys of one column per lane).
+// (ds_read_b64_tr_b16: 4 keys of one column per lane). Two workgroups to a CU (256 registers a lane): the one's exponentials run
+// beside the other's products, and within a wave beside the next tile's first product.
+// Measured: 509 tokens behind 32003 keys (32 query, 4 key heads of 128) 275 us and the join's 10, 0.98 PFLOP/s in the kernel, where a
+// large bf16 product reaches 1.38; three prompts of 5092 tokens 107 us, 0.70 PFLOP/s with its ramp and tail. Sequences of 17 to 32
+// rows are better off here than as two sets of the kernel above: 64 users of 4 tokens behind 2048 keys 68 us, there 109.
 constexpr int kTileWaves = 4;
 static_assert(kTileRows == 32 * kTileWaves, "a wave has 32 rows");
 
@@ -704,6 +714,9 @@ __global__ __launch_bounds__(64 * kTileWaves, D <= 128 ? 2 : 1) void attend_tile
                     o[j] = M::mma32(a, pr, o[j]);
                 }
             }
+        // The order: six operands of the first product ahead, then each of its instructions with two exponentials and their company; the
+        // second product's operands one instruction ahead. Left to itself 297 us (509 tokens behind 32003), in this order 264; operands
+        // read just ahead of each instruction 360.
         if constexpr (decltype(more)::value && D <= 128) {
             __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll

@@ -7,13 +7,15 @@
 // about its mean; one wave per row needs no barrier. Wider rows take one workgroup each and read the row again from L2.
 // Backward keeps the columns' sums of dw and db in registers over the rows that a lane sees, adds the rows of a workgroup through LDS
 // in order and writes one partial row per workgroup; a second launch adds those in order: no atomics, the same bits every run.
+// Measured on 16384 rows of 2880 in bf16: forward 36 us, 5.2 TB/s, the rate of a large copy; backward 70 us, 4.1 TB/s, and 4 us for
+// the partial rows. 5003 rows of 1111 in fp32 with a bias: 13, 21 and 4 us. One row of 2048: 3.3 us, bound by latency.
 #include "layer_common.h"
 
 namespace cmoe {
 
 constexpr int kWaves = 8;       // of a workgroup, shared out over its rows
 constexpr int kRowChunks = 4;   // vectors of a row per lane, forward
-constexpr int kBackChunks = 3;  // backward: two rows' vectors and two sums per column; 128 registers leave 16 waves to a CU
+constexpr int kBackChunks = 3;  // backward: two rows' vectors, one or two sums per column; 128 registers leave 16 waves to a CU (at 151: 103 us, at 128: 70)
 constexpr int kWideThreads = 1024;
 
 // Vector c of a row, zeros past its end.
