@@ -213,7 +213,7 @@ __device__ __forceinline__ float row_scale(const AttentionParams& p, int head, f
     return l > 0.0f || l != l ? 1.0f / l : 0.0f;  // a row that sees nothing is 0
 }
 
-__device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
+__device__ const __align__(16) uint32_t kZeros[4] = {0, 0, 0, 0};
 
 // ---- few rows: single tokens and short chunks ---------------------------------------------------------------------------------
 // Bound by the stream of keys and values. The four waves of a workgroup share out its keys, and each runs alone: 16 keys at a time

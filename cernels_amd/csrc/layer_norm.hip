@@ -94,9 +94,9 @@ __global__ __launch_bounds__(64 * kWaves) void norm_row_kernel(NormParams p, int
 #pragma unroll
         for (int i = 0; i < V; ++i) sum[0] += f[i];
     }
-    const float inv = 1.0f / (float)p.cols;
+    const float n = (float)p.cols;  // divided by, so that a row of one value has exactly that mean
     row_sum<1>(sum, gw, lds[0]);
-    const float mean = sum[0] * inv;
+    const float mean = sum[0] / n;
     sum[0] = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(64 * kWaves) void norm_row_kernel(NormParams p, int
         }
     }
     row_sum<1>(sum, gw, lds[1]);
-    const float rstd = 1.0f / sqrtf(sum[0] * inv + p.eps);
+    const float rstd = 1.0f / sqrtf(sum[0] / n + p.eps);
     if (p.stats && first == 0 && cols) p.stats[2 * row] = mean, p.stats[2 * row + 1] = rstd;
     typename T::raw* y = static_cast<typename T::raw*>(p.y) + row * cols;
 #pragma unroll
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_wide_kernel(NormParams p) {
     constexpr int V = T::kVec;
     __shared__ float lds[kWideThreads / 64];
     const int cols = p.cols, chunks = ceil_div(cols, V);
-    const float inv = 1.0f / (float)cols;
+    const float n = (float)cols;
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const typename T::raw* x = static_cast<const typename T::raw*>(p.x) + row * cols;
         float s[1] = {0.0f};
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_wide_kernel(NormParams p) {
             for (int i = 0; i < V; ++i) s[0] += f[i];
         }
         block_sum<1>(s, lds);
-        const float mean = s[0] * inv;
+        const float mean = s[0] / n;
         s[0] = 0.0f;
         for (int c = threadIdx.x; c < chunks; c += kWideThreads) {
             float f[V];
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_wide_kernel(NormParams p) {
             }
         }
         block_sum<1>(s, lds);
-        const float rstd = 1.0f / sqrtf(s[0] * inv + p.eps);
+        const float rstd = 1.0f / sqrtf(s[0] / n + p.eps);
         if (p.stats && threadIdx.x == 0) p.stats[2 * row] = mean, p.stats[2 * row + 1] = rstd;
         typename T::raw* y = static_cast<typename T::raw*>(p.y) + row * cols;
         for (int c = threadIdx.x; c < chunks; c += kWideThreads) {

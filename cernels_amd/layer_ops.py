@@ -432,7 +432,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     seqs, blocks, page_size = block_table.size(0), block_table.size(1), k_pages.size(1)
     if tokens and seqs:
         L = _native.lib()
-        most = int(max_new) if max_new is not None else 0
+        # of a sequence's new tokens; 0: not known
+        most = tokens // seqs if q_offsets is None else int(max_new) if max_new is not None else 0
         nbytes = L.cernels_paged_attention_workspace_bytes(tokens, seqs, heads, kv_heads, dim, page_size, blocks, most)
         if nbytes == 0:
             raise RuntimeError(f"cernels_paged_attention: invalid dimensions tokens={tokens} heads={heads}/{kv_heads} dim={dim} "

@@ -329,7 +329,8 @@ int cernels_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_s
  * first). The query at position p sees keys j <= p, with window > 0 also j > p - window; query head h reads key head
  * h / (heads / kv_heads); softmax of scale * q k in fp32; sinks [heads] fp32 (nullable) is one more logit of each head without a
  * value. A row that sees nothing is 0. out [tokens, heads, dim] contiguous. max_new: the most new tokens that any sequence has, or
- * 0 if unknown; it steers the choice of kernels only, results hold for any value. Values (V) of keys past the sequence's length
+ * 0 if unknown; it steers the choice of kernels only, results hold for any value. The workspace is that of the same tokens, seqs
+ * and max_new (tokens / seqs where q_offsets is NULL). Values (V) of keys past the sequence's length
  * or before every window of the step may hold anything.
  * Limits: dim 64, 128 or 256; heads % kv_heads == 0; page_strides multiples of 8, the slots' under 2^26, pages 16-byte
  * aligned; scale > 0. */

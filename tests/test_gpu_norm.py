@@ -179,3 +179,22 @@ def test_captured_training_step_replays(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(kept, want)), i
+
+
+def test_more_than_2_31_elements(device):
+    rows, cols = 1_050_000, 2053
+    assert rows * cols > 2 ** 31
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=device)
+    g = torch.Generator(device=device).manual_seed(5)
+    tail = torch.randn(7, cols, generator=g, device=device).bfloat16()
+    x[:-7], x[-7:] = 1.0, tail
+    w = torch.randn(cols, generator=g, device=device).bfloat16()
+    y = ops.layer_norm(x, w)
+    assert torch.equal(y[-7:], ops.layer_norm(tail, w)) and not y[:3].any()
+    del y
+    x.requires_grad_()
+    dy = torch.ones(1, cols, dtype=torch.bfloat16, device=device).expand(rows, cols).contiguous()
+    (dx,) = torch.autograd.grad(ops.layer_norm(x, w), x, dy)
+    leaf = tail.clone().requires_grad_()
+    (want,) = torch.autograd.grad(ops.layer_norm(leaf, w), leaf, dy[-7:])
+    assert torch.equal(dx[-7:], want)

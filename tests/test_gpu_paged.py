@@ -154,6 +154,17 @@ def test_uniform_steps_without_offsets(device):
         check(s, call(s, q_offsets=None))
 
 
+@pytest.mark.parametrize("n,count", [(1, 70), (1, 300), (5, 64), (20, 9)])
+def test_many_uniform_sequences_without_offsets(device, n, count):
+    """The workspace is the one of the kernels that a uniform step takes, whether the caller names its length or not."""
+    g = torch.Generator().manual_seed(count)
+    s = make_step([(n, n + int(torch.randint(0, 700, (1,), generator=g))) for _ in range(count)], 8, 2, 64, 16, torch.bfloat16, device, blocks=300)
+    want = call(s, q_offsets=None)
+    check(s, want)
+    for most in (None, 1, n, 10 * n):
+        assert torch.equal(call(s, q_offsets=None, max_new=most), want)
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_pages_in_other_orders(device, new):
     """Pages as [pages, heads, slots, dim], queries as a slice of a fused projection, a table that is a slice of a wider one."""

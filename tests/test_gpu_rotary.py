@@ -135,3 +135,13 @@ def test_captured_call_replays(device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(kept, want), i
+
+
+def test_more_than_2_31_elements(device):
+    tokens = 263_000
+    q = torch.empty(tokens, 64, 128, dtype=torch.bfloat16, device=device)
+    assert q.numel() > 2 ** 31
+    q[-5:].normal_()
+    pos, inv = torch.arange(tokens, device=device), ops.rotary_frequencies(128, device=device)[0]
+    y, _ = ops.rotary(q, None, pos, inv, interleaved=True)
+    assert_turned(y[-5:], q[-5:], pos[-5:], inv, True)
