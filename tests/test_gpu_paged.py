@@ -142,6 +142,41 @@ def test_long_cache_splits_and_joins(device):
         check(s, call(s, window=2500), window=2500)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new", [1, 60])
+def test_one_key_over_a_long_flat_rest(device, new, dtype):
+    """One key has e^11 times the weight of each of the 9000 others, which together still weigh 0.15 of it: probabilities of 2^-16, below
+    fp16's normal numbers. Bound: as everywhere, and 2^-25 for each such probability (half of fp16's smallest step) against the sum of
+    the weights, times max |v|."""
+    s = make_step([(new, 9000)], 2, 1, 64, 64, dtype, device, seed=new)
+    q = torch.zeros_like(s["q"])
+    q[..., 0] = 8.0
+    s["q"] = q
+    k = torch.zeros(9000, 1, 64, dtype=dtype)
+    k[4000, 0, 0] = 11.0
+    s["keys"][0] = k
+    j = torch.arange(9000, device=device)
+    s["k_pages"][s["block_table"][0, j // 64].long(), j % 64] = k.to(device)
+    for scale in (0.125, 0.17):
+        got = call(s, scale=scale).double().cpu()
+        want, tol = exact_attention(s, scale=scale)
+        tol = tol + 9000 * 2.0 ** -25 * float(s["values"][0].abs().max())
+        assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+def test_small_values(device):
+    """Values below fp16's smallest normal number keep their own precision: steps of 2^-24."""
+    for new in (1, 40):
+        s = make_step([(new, 200)], 4, 1, 64, 16, torch.float16, device, seed=new)
+        small = (s["values"][0].double() * 2.0 ** -17).half()
+        s["values"][0] = small
+        j = torch.arange(200, device=device)
+        s["v_pages"][s["block_table"][0, j // 16].long(), j % 16] = small.to(device)
+        got = call(s).double().cpu()
+        want, tol = exact_attention(s)
+        assert ((got - want).abs() <= tol + 2.0 ** -25).all()
+
+
 def test_wrong_max_new_changes_nothing(device):
     s = make_step([(90, 300), (1, 50), (300, 310)], 8, 2, 128, 16, torch.bfloat16, device)
     for most in (1, 2, 10, 100, 10_000):
