@@ -272,32 +272,17 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttentionPar
     for (int r0 = 0; r0 < rows; r0 += 16) {
         // rows r0 .. r0 + 15: this lane's, its query and the keys that they see
         u32x4 q[DS];
-        int most_hi = 0, least_lo = 0x7fffffff, all_hi = 0x7fffffff, all_lo = 0;
-        const int row = r0 + col;
+        const int row = r0 + col, last = min(r0 + 15, rows - 1), before = length - count;
         const bool live = row < rows;
         const int token = live ? row / group : 0, head = kh * group + (live ? row - token * group : 0);
         const raw* src = static_cast<const raw*>(p.q.p) + (first + token) * p.q.token + head * p.q.head;
 #pragma unroll
         for (int s = 0; s < DS; ++s) q[s] = live ? load_vec<T>(src + 8 * (g + 4 * s)) : u32x4{};
-        const int pos = length - count + token;
-        const int hi = live ? pos + 1 : 0, lo = p.window > 0 && pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
-        if (live) {
-            most_hi = max(most_hi, hi);
-            least_lo = min(least_lo, lo);
-            all_hi = min(all_hi, hi);
-            all_lo = max(all_lo, lo);
-        }
-#pragma unroll
-        for (int o = 8; o; o >>= 1) {
-            most_hi = max(most_hi, __shfl_xor(most_hi, o));
-            least_lo = min(least_lo, __shfl_xor(least_lo, o));
-            all_hi = min(all_hi, __shfl_xor(all_hi, o));
-            all_lo = max(all_lo, __shfl_xor(all_lo, o));
-        }
-        most_hi = __builtin_amdgcn_readfirstlane(min(most_hi, p.step.blocks * page_size));
-        least_lo = __builtin_amdgcn_readfirstlane(least_lo);
-        all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-        all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+        // positions grow with the row: the first row sees the fewest later keys, the last one the fewest earlier ones
+        auto low = [&](int tok) __attribute__((always_inline)) { return p.window > 0 && before + tok - p.window + 1 > 0 ? before + tok - p.window + 1 : 0; };
+        const int hi = live ? before + token + 1 : 0, lo = low(token);
+        const int all_hi = before + r0 / group + 1, least_lo = low(r0 / group), all_lo = low(last / group);
+        const int most_hi = min(max(before + last / group + 1, 0), p.step.blocks * page_size);
         int begin, end;
         split_range(least_lo & ~(kFewKeys - 1), most_hi, split, t.parts, kFewKeys * kFewWaves, begin, end);
         // this wave's quarter of them; a stage lies inside one page (pages hold a multiple of 16 slots), and the pages are walked along
@@ -843,11 +828,21 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttentionParams p, Att
     constexpr int E = D / 64;
     const int lane = threadIdx.x & 63;
     const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int token = (int)(at / p.q.heads), head = (int)(at - (long long)token * p.q.heads);
-    if (token >= p.step.tokens) return;
-    if (step_sequence(p.step, token) >= p.step.seqs) return;
+    if (at >= (long long)p.step.tokens * p.q.heads) return;
+    const int token = (int)at / p.q.heads, head = (int)at - token * p.q.heads;  // fewer than 2^31 rows
+    // what the row needs is on its way before it is known to be one: every row has its place in the workspace
     const float2* st = plan_stats(plan, p) + at * plan.splits;
     const float2 mine = lane < plan.splits ? st[lane] : make_float2(kNone, 0.0f);
+    const float* part = plan.part + at * plan.splits * D + E * lane;
+    float v[4][E];
+    auto fetch = [&](int i, int n) __attribute__((always_inline)) {  // four splits at a time
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[u][e] = part[(long long)min(i + u, n - 1) * D + e];
+    };
+    fetch(0, plan.splits);
+    if (step_sequence(p.step, token) >= p.step.seqs) return;
     const float mx = wave_max(mine.y == 0.0f ? kNone : mine.x);
     const float f = mine.y == 0.0f || mine.x == kNone ? 0.0f : __builtin_amdgcn_exp2f(mine.x - mx);
     const float sum = wave_sum(f * mine.y);
@@ -856,13 +851,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttentionParams p, Att
     float o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
-    const float* part = plan.part + at * plan.splits * D + E * lane;
-    for (int i = 0; i < n; i += 4) {  // four at a time are on their way
-        float v[4][E];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[u][e] = part[(long long)min(i + u, n - 1) * D + e];
+    for (int i = 0; i < n; i += 4) {
+        if (i) fetch(i, n);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const float w = i + u < n ? __shfl(f, i + u) : 0.0f;
