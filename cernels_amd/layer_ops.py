@@ -51,6 +51,17 @@ def _refuse_gradient(what, *tensors) -> None:
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
 
 
+def _once(backward):
+    """A backward pass whose gradients have none of their own: differentiating them raises. Only a graph of the gradients needs the
+    wrapper that says so; without one (gradients are computed with grad mode off) its 4 us on autograd's thread are left out."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def entry(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return entry
+
+
 # ---- layer norm ---------------------------------------------------------------------------------------------------------
 
 
@@ -84,7 +95,7 @@ def _norm_forward(x, weight, bias, eps, keep_stats):
     cols = x.size(-1)
     rows = x.numel() // cols
     y = torch.empty_like(x)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if keep_stats else None
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if keep_stats else None
     if rows:
         _launch("cernels_layer_norm", x.get_device(), _native.lib().cernels_layer_norm, x.data_ptr(), weight.data_ptr(), _ptr(bias),
                 rows, cols, _DTYPES[x.dtype], _DTYPES[weight.dtype], eps, y.data_ptr(), _ptr(stats))
@@ -99,22 +110,21 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        cols = x.size(-1)
-        rows = x.numel() // cols
+        rows, cols = stats.size(0), x.size(-1)
         dy = dy.contiguous()
         dx = torch.empty_like(x) if want_x else None
         dw = torch.empty_like(weight) if want_w else None
         db = torch.empty_like(weight) if want_b else None
-        L = _native.lib()
-        nbytes = L.cernels_layer_norm_backward_workspace_bytes(rows, cols, _DTYPES[x.dtype]) if want_w or want_b else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        L, dtype = _native.lib(), _DTYPES[x.dtype]
+        nbytes = L.cernels_layer_norm_backward_workspace_bytes(rows, cols, dtype) if want_w or want_b else 0
+        ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _launch("cernels_layer_norm_backward", x.get_device(), L.cernels_layer_norm_backward, dy.data_ptr(), x.data_ptr(),
-                weight.data_ptr(), stats.data_ptr(), rows, cols, _DTYPES[x.dtype], _DTYPES[weight.dtype], _ptr(dx), _ptr(dw),
-                _ptr(db), ws.data_ptr(), nbytes)
+                weight.data_ptr(), stats.data_ptr(), rows, cols, dtype, _DTYPES[weight.dtype], _ptr(dx), _ptr(dw), _ptr(db),
+                _ptr(ws), nbytes)
         return dx, dw, db, None
 
 
@@ -243,7 +253,7 @@ class _Rotary(torch.autograd.Function):
         return tuple(_rotary_launch(q, k, positions, inv_freq, interleaved, scale, 0))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         grads = [t if want else None for t, want in zip((dq, dk), ctx.needs_input_grad)]

@@ -198,3 +198,14 @@ def test_more_than_2_31_elements(device):
     leaf = tail.clone().requires_grad_()
     (want,) = torch.autograd.grad(ops.layer_norm(leaf, w), leaf, dy[-7:])
     assert torch.equal(dx[-7:], want)
+
+
+def test_gradients_have_no_gradients(device):
+    x, w, b, dy = (t.to(device) for t in _case(7, 96, torch.float32, torch.float32, True))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    plain = torch.autograd.grad(ops.layer_norm(*leaves), leaves, dy)
+    graphed = torch.autograd.grad(ops.layer_norm(*leaves), leaves, dy.clone().requires_grad_(), create_graph=True)
+    for a, c in zip(plain, graphed):
+        assert torch.equal(a, c)
+        with pytest.raises(RuntimeError, match="differentia"):
+            c.sum().backward(retain_graph=True)

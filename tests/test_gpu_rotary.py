@@ -145,3 +145,14 @@ def test_more_than_2_31_elements(device):
     pos, inv = torch.arange(tokens, device=device), ops.rotary_frequencies(128, device=device)[0]
     y, _ = ops.rotary(q, None, pos, inv, interleaved=True)
     assert_turned(y[-5:], q[-5:], pos[-5:], inv, True)
+
+
+def test_gradients_have_no_gradients(device):
+    q = torch.randn(5, 3, 64, device=device, requires_grad=True)
+    pos, inv = torch.arange(5, device=device), ops.rotary_frequencies(64, device=device)[0]
+    dy = torch.randn_like(q)
+    plain, = torch.autograd.grad(ops.rotary(q, None, pos, inv)[0], q, dy)
+    graphed, = torch.autograd.grad(ops.rotary(q, None, pos, inv)[0], q, dy.clone().requires_grad_(), create_graph=True)
+    assert torch.equal(plain, graphed)
+    with pytest.raises(RuntimeError, match="differentia"):
+        graphed.sum().backward()
